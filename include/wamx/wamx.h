@@ -52,13 +52,22 @@ extern "C" {
 
 /* ---------------------------------------------------------------------------
  * Enums.  Values of wamx_type follow enum ggml_type (F32=0, F16=1, I32=26,
- * BF16=30).  wamx_status follows enum ggml_status.
+ * BF16=30, MXFP4=39).  wamx_status follows enum ggml_status.
  * ------------------------------------------------------------------------- */
 typedef enum wamx_type {
     WAMX_TYPE_F32  = 0,
     WAMX_TYPE_F16  = 1,
     WAMX_TYPE_I32  = 26,
     WAMX_TYPE_BF16 = 30,
+    /* Microscaled 4-bit floating point (OCP MX v1.0, e2m1 elements): a row is
+     * blocks of 32 values in 17 bytes, byte 0 the biased exponent e of the
+     * block's scale 2^(e - 127) (255: every value NaN), byte 1 + j the codes of
+     * value j (low half) and value j + 16 (high half): sign, two exponent bits,
+     * one mantissa bit, {0, .5, 1, 1.5, 2, 3, 4, 6}.  The layout of ggml's
+     * block_mxfp4.  ne[0] is a multiple of 32, nb[0] = 17 the bytes of a block.
+     * Read by MUL_MAT and LINEAR (as the weight), GET_ROWS and CPY; written by
+     * CPY. */
+    WAMX_TYPE_MXFP4 = 39,
 } wamx_type;
 
 typedef enum wamx_status {
@@ -101,6 +110,8 @@ typedef enum wamx_op {
     WAMX_OP_MODULATION,       /* CAST(f32) + ADD of the adaLN modulation and table */
     WAMX_OP_EULER_STEP,       /* CAST(f32) x2 + MUL(dt) + ADD + CAST(bf16): scheduler_step */
     WAMX_OP_MLP_SMALL,        /* [GELU_ERF] + (MUL_MAT + ADD bias [+ GELU_ERF]) x2, widths <= 128 */
+    WAMX_OP_HEAD_NORM_ROPE,   /* RMS_NORM per head + ROPE + CAST(bf16) + append to a cache; V^T append */
+    WAMX_OP_TREE_ATTN,        /* attention of a tree of drafted tokens over a cache */
     WAMX_OP_COUNT
 } wamx_op;
 
@@ -163,7 +174,8 @@ typedef struct wamx_cgraph  wamx_cgraph;
 WAMX_API wamx_context * wamx_init(size_t max_tensors);
 WAMX_API void           wamx_free(wamx_context * ctx);
 
-WAMX_API size_t  wamx_type_size(int32_t type);
+WAMX_API size_t  wamx_type_size(int32_t type);   /* bytes of an element, or of a block (MXFP4: 17) */
+WAMX_API int64_t wamx_blck_size(int32_t type);   /* elements of a block (MXFP4: 32, else 1) */
 WAMX_API const char * wamx_type_name(int32_t type);
 WAMX_API const char * wamx_op_name(int32_t op);
 WAMX_API int64_t wamx_nelements(const wamx_tensor * t);
@@ -312,6 +324,31 @@ WAMX_API wamx_tensor * wamx_rms_norm_bf16_f32(wamx_context * ctx, wamx_tensor * 
  *   W1 bf16 [ne={K0, M1}], b1 bf16 [M1], W2 bf16 [ne={M1, M2}], b2 bf16 [M2];
  *   y bf16 [ne={M2, N}].  Each GELU_ERF rounds to bf16.  fp32 accumulation
  *   (in k order).
+ *
+ * wamx_qk_head_norm_rope: RMSNorm of every head of x bf16 [ne={dh*H, T*B}] (row
+ *   stride nb[1], for example the query or key columns of a packed projection)
+ *   over its dh values times weight bf16 [dh], rotation of the first n_dims
+ *   values by pos I32 [T*B] (pair i by pos * freq_base^(-2i / n_dims);
+ *   rope_mode 0 pairs neighbours, 2 pairs the halves; n_dims 0: none) and the
+ *   result, rounded to bf16 once, into dst bf16 [ne={dh, rows, H, B}]: token t
+ *   of sequence b in slot past[b] + t (past I32 [B], NULL: 0).  A slot outside
+ *   [0, rows) is not written.  dh 64, 128 or 256, n_dims a multiple of 16.
+ *   wamx_qk_norm_rope differs in that it norms over the whole row.
+ * wamx_vt_append: the values x bf16 [ne={dh*H, T*B}] into the same slots of a
+ *   transposed cache dst bf16 [ne={rows, dh, H, B}] (row stride nb[1]).
+ *   Both return a view of dst that depends on the write; pass it on to the
+ *   node that reads the cache.
+ *
+ * wamx_tree_attn: softmax(scale q.k) v of T drafted tokens per sequence over a
+ *   resident cache.  q bf16 [ne={dh, T, H, B}], k bf16 [ne={dh, rows, KV, B}],
+ *   v bf16 [ne={rows, dh, KV, B}] (V^T, row stride a multiple of 8 values),
+ *   H a multiple of KV (query head h reads key head h / (H / KV)).  Sequence
+ *   b's cache holds past[b] slots (I32 [B], NULL: 0) that every token sees, and
+ *   its drafted tokens in the T slots behind them; token i sees itself and its
+ *   ancestors: parents I32 [T, B] holds each token's parent, -1 at the root.
+ *   Any other value outside [0, T) marks a slot without a token: nothing sees
+ *   it and its result is zero.  A sequence whose past[b] is outside
+ *   [0, rows - T] gets zeros.  T 1 to 256.  Output bf16 [ne={dh*H, T, B}].
  */
 WAMX_API wamx_tensor * wamx_linear(wamx_context * ctx, wamx_tensor * w, wamx_tensor * x, wamx_tensor * bias,
                                    int32_t epilogue, wamx_tensor * residual, wamx_tensor * gate);
@@ -321,6 +358,12 @@ WAMX_API wamx_tensor * wamx_qk_norm_rope(wamx_context * ctx, wamx_tensor * x, wa
 WAMX_API wamx_tensor * wamx_joint_attn(wamx_context * ctx, wamx_tensor * q, wamx_tensor * k_a, wamx_tensor * v_a,
                                        wamx_tensor * k_b, wamx_tensor * v_b, int64_t na_split, float scale);
 WAMX_API wamx_tensor * wamx_modulation(wamx_context * ctx, wamx_tensor * mod, wamx_tensor * tables);
+WAMX_API wamx_tensor * wamx_qk_head_norm_rope(wamx_context * ctx, wamx_tensor * x, wamx_tensor * weight,
+                                              wamx_tensor * dst, wamx_tensor * past, wamx_tensor * pos,
+                                              int rope_mode, int n_dims, float eps, float freq_base);
+WAMX_API wamx_tensor * wamx_vt_append(wamx_context * ctx, wamx_tensor * x, wamx_tensor * dst, wamx_tensor * past);
+WAMX_API wamx_tensor * wamx_tree_attn(wamx_context * ctx, wamx_tensor * q, wamx_tensor * k, wamx_tensor * v,
+                                      wamx_tensor * parents, wamx_tensor * past, float scale);
 WAMX_API wamx_tensor * wamx_qk_norm_rope_hilo(wamx_context * ctx, wamx_tensor * x, wamx_tensor * weight,
                                               wamx_tensor * dst, int64_t tok0, int rope_mode, wamx_tensor * pos0,
                                               wamx_tensor * pos1, wamx_tensor * pos2, float eps, float freq_base);
@@ -574,6 +617,43 @@ WAMX_API wamx_status wamx_op_rope_table(wamx_backend_t be, int rope_mode, const 
 WAMX_API wamx_status wamx_op_qk_norm_rope_table(wamx_backend_t be, const void * x, int64_t ldx, const void * w,
                                                 void * dst, int64_t heads, int64_t head_dim, int64_t tokens,
                                                 int64_t dst_tokens, int64_t tok0, const float * table, float eps);
+/* MXFP4 rows (see WAMX_TYPE_MXFP4), packed one after another: cols / 32 * 17
+ * bytes each, cols a multiple of 32.  quantize: x f32, f16 or bf16, row stride
+ * ldx.  Scale exponent floor(log2 max|x|) - 2 of each block (at least -127, the
+ * scale of a block of zeros as well), values to the nearest code, halves to the
+ * even one, 6 the largest; a block with an Inf or NaN becomes NaN (scale byte
+ * 255).  dequantize: the values, rounded to y's type. */
+WAMX_API wamx_status wamx_op_quantize_mxfp4(wamx_backend_t be, const void * x, int32_t x_type, int64_t ldx, void * q,
+                                            int64_t rows, int64_t cols);
+WAMX_API wamx_status wamx_op_dequantize_mxfp4(wamx_backend_t be, const void * q, void * y, int32_t y_type, int64_t ldy,
+                                              int64_t rows, int64_t cols);
+/* wamx_op_mul_mat and wamx_op_linear with w in MXFP4 rows [M][K], K a multiple
+ * of 32: x (bf16, or f32 rounded to bf16), f32 accumulation, any N. */
+WAMX_API wamx_status wamx_op_mul_mat_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type, int64_t ldx,
+                                           void * y, int32_t y_type, int64_t ldy, int64_t M, int64_t N, int64_t K);
+WAMX_API wamx_status wamx_op_linear_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type,
+                                          const void * bias, int32_t epilogue, const void * residual,
+                                          const float * gate, void * y, int64_t M, int64_t N, int64_t K);
+/* wamx_qk_head_norm_rope of queries and keys and wamx_vt_append in one launch,
+ * from packed rows x bf16 [batch * tokens][ldx] of heads * head_dim query,
+ * kv_heads * head_dim key and kv_heads * head_dim value columns.
+ * q [batch][heads][tokens][head_dim], k [batch][kv_heads][capacity][head_dim],
+ * vt [batch][kv_heads][head_dim][vt_ld].  A NULL q, k or vt leaves that part
+ * out (its columns are there all the same).  wq, wk [head_dim]; pos
+ * [batch * tokens]; past [batch] (NULL: 0). */
+WAMX_API wamx_status wamx_op_qkv_head_norm_rope(wamx_backend_t be, const void * x, int64_t ldx, const void * wq,
+                                                const void * wk, const int32_t * pos, const int32_t * past, void * q,
+                                                void * k, void * vt, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t tokens, int64_t batch, int64_t capacity,
+                                                int64_t vt_ld, int rope_mode, int n_dims, float eps, float freq_base);
+/* wamx_tree_attn on device pointers: q [batch][heads][tokens][head_dim],
+ * k [batch][kv_heads][capacity][head_dim], vt [batch][kv_heads][head_dim][vt_ld]
+ * (vt_ld % 8 == 0; q, k and vt 16-byte aligned), parents [batch][tokens], past
+ * [batch] (NULL: 0), out bf16 [batch][tokens][heads * head_dim]. */
+WAMX_API wamx_status wamx_op_tree_attn(wamx_backend_t be, const void * q, const void * k, const void * vt,
+                                       const int32_t * parents, const int32_t * past, void * out, int64_t heads,
+                                       int64_t kv_heads, int64_t head_dim, int64_t tokens, int64_t batch,
+                                       int64_t capacity, int64_t vt_ld, float scale);
 /* SOFT_MAX_EXT without mask: y[r][:] = softmax(scale * x[r][:]) over ne0=cols, f32. */
 WAMX_API wamx_status wamx_op_soft_max_f32(wamx_backend_t be, const float * x, float * y,
                                           int64_t rows, int64_t cols, float scale);
@@ -879,7 +959,7 @@ WAMX_API int32_t      wamx_ggml_op_to_wamx(int i);
  * ggml_tensor fields, with names instead of enum values:
  *   op       = ggml_op_name(t->op)            ("NONE" for leaves)
  *   unary_op = ggml_unary_op_name(ggml_get_unary_op(t)) for UNARY, else NULL
- *   type     = ggml_type_name(t->type)        ("f32", "f16", "bf16", "i32")
+ *   type     = ggml_type_name(t->type)        ("f32", "f16", "bf16", "i32", "mxfp4")
  *   ne, nb, op_params, flags, data, name      copied verbatim
  *   src[i], view_src                           indices into the array, -1 = none
  * op_params are read in ggml's layouts (ROPE, SOFT_MAX, SCALE, IM2COL, NORM,

@@ -261,7 +261,134 @@ static GemmArgs mul_mat_args(wamx_backend * be, const wamx_tensor * node) {
     return g;
 }
 
+static bool is_mxfp4(const wamx_tensor * t) { return t && t->type == WAMX_TYPE_MXFP4; }
+
+// Whether the planes of t (dims 2 and 3) continue its rows, so that all of
+// them are rows of one matrix.
+static bool planes_fold(const wamx_tensor * t) {
+    return (t->ne[2] == 1 || t->nb[2] == t->nb[1] * (size_t) t->ne[1]) &&
+           (t->ne[3] == 1 || t->nb[3] == t->nb[1] * (size_t) (t->ne[1] * t->ne[2]));
+}
+
+// MUL_MAT with a weight in MXFP4: one product where one weight meets rows that
+// follow each other, else one per plane.
+static hipError_t run_mxfp4_mul_mat(wamx_backend * be, const wamx_tensor * node) {
+    const wamx_tensor *w = node->src[0], *x = node->src[1];
+    MxArgs a;
+    a.w_stride = (int64_t) w->nb[1];
+    a.x_type = x->type;
+    a.ldx = (int64_t) x->nb[1] / es(x);
+    a.y_type = node->type;
+    a.ldy = (int64_t) node->nb[1] / es(node);
+    a.M = w->ne[1];
+    a.K = w->ne[0];
+    a.ws = be->cws;
+    a.ws_bytes = kWorkspaceBytes;
+    const bool one = w->ne[2] == 1 && w->ne[3] == 1 && planes_fold(x);
+    a.N = one ? x->ne[1] * x->ne[2] * x->ne[3] : x->ne[1];
+    for (int64_t i3 = 0; i3 < (one ? 1 : x->ne[3]); ++i3)
+        for (int64_t i2 = 0; i2 < (one ? 1 : x->ne[2]); ++i2) {
+            const int64_t w2 = i2 / (x->ne[2] / w->ne[2]), w3 = i3 / (x->ne[3] / w->ne[3]);
+            a.w = (const char *) w->data + w2 * w->nb[2] + w3 * w->nb[3];
+            a.x = (const char *) x->data + i2 * x->nb[2] + i3 * x->nb[3];
+            a.y = (char *) node->data + i2 * node->nb[2] + i3 * node->nb[3];
+            const hipError_t e = launch_mx_product(a, be->cs);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+
+static hipError_t run_mxfp4_linear(wamx_backend * be, const wamx_tensor * node) {
+    const wamx_tensor *w = node->src[0], *x = node->src[1], *res = node->src[3];
+    MxArgs a;
+    a.w = w->data;
+    a.w_stride = (int64_t) w->nb[1];
+    a.x = x->data;
+    a.x_type = x->type;
+    a.ldx = (int64_t) x->nb[1] / es(x);
+    a.y = node->data;
+    a.ldy = (int64_t) node->nb[1] / 2;
+    a.M = w->ne[1];
+    a.N = x->ne[1];
+    a.K = w->ne[0];
+    a.epi = node->op_params[0];
+    a.bias = node->src[2] ? node->src[2]->data : nullptr;
+    a.res = res ? res->data : nullptr;
+    a.ldres = res ? (int64_t) res->nb[1] / 2 : 0;
+    a.gate = node->src[4] ? (const float *) node->src[4]->data : nullptr;
+    a.ws = be->cws;
+    a.ws_bytes = kWorkspaceBytes;
+    return launch_mx_product(a, be->cs);
+}
+
+// CPY to or from MXFP4, plane by plane where the strided side does not fold.
+static hipError_t run_mxfp4_copy(wamx_backend * be, const wamx_tensor * src, const wamx_tensor * dst) {
+    const bool to = is_mxfp4(dst), one = planes_fold(src) && planes_fold(dst);
+    const int64_t rows = one ? wamx_nrows(src) : src->ne[1], cols = src->ne[0];
+    for (int64_t i3 = 0; i3 < (one ? 1 : src->ne[3]); ++i3)
+        for (int64_t i2 = 0; i2 < (one ? 1 : src->ne[2]); ++i2) {
+            const char * s = (const char *) src->data + i2 * src->nb[2] + i3 * src->nb[3];
+            char * d = (char *) dst->data + i2 * dst->nb[2] + i3 * dst->nb[3];
+            const hipError_t e =
+                to ? launch_mx_quantize(s, src->type, (int64_t) src->nb[1] / es(src), d, rows, cols, be->cs)
+                   : launch_mx_dequantize(s, (int64_t) src->nb[1], nullptr, 0, d, dst->type,
+                                          (int64_t) dst->nb[1] / es(dst), rows, cols, be->cs);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+
+static hipError_t run_head_norm_rope(wamx_backend * be, const wamx_tensor * node) {
+    const wamx_tensor *x = node->src[0], *dst = node->src[2];
+    const bool vt = node->op_params[4] != 0;
+    HeadNormArgs a;
+    a.x = x->data;
+    a.ldx = (int64_t) x->nb[1] / 2;
+    a.past = node->src[3] ? (const int32_t *) node->src[3]->data : nullptr;
+    a.batch = dst->ne[3];
+    a.tokens = x->ne[1] / a.batch;
+    a.head_dim = dst->ne[vt ? 1 : 0];
+    a.k_rows = dst->ne[vt ? 0 : 1];
+    a.kv_heads = dst->ne[2];
+    if (vt) {
+        a.vt = dst->data;
+        a.vt_ld = (int64_t) dst->nb[1] / 2;
+    } else {
+        a.wk = node->src[1]->data;
+        a.k = dst->data;
+        a.rope_mode = node->op_params[0];
+        a.n_dims = node->op_params[1];
+        memcpy(&a.eps, &node->op_params[2], 4);
+        memcpy(&a.freq_base, &node->op_params[3], 4);
+        a.pos = a.n_dims > 0 ? (const int32_t *) node->src[4]->data : nullptr;
+    }
+    return launch_head_norm_rope(a, be->cs);
+}
+
+static hipError_t run_tree_attn(wamx_backend * be, const wamx_tensor * node) {
+    const wamx_tensor *q = node->src[0], *k = node->src[1], *v = node->src[2];
+    TreeArgs a;
+    a.q = q->data;
+    a.k = k->data;
+    a.vt = v->data;
+    a.parents = (const int32_t *) node->src[3]->data;
+    a.past = node->src[4] ? (const int32_t *) node->src[4]->data : nullptr;
+    a.out = node->data;
+    a.heads = q->ne[2];
+    a.kv_heads = k->ne[2];
+    a.head_dim = q->ne[0];
+    a.tq = q->ne[1];
+    a.batch = q->ne[3];
+    a.capacity = k->ne[1];
+    a.vt_ld = (int64_t) v->nb[1] / 2;
+    memcpy(&a.scale, &node->op_params[0], 4);
+    a.ws = be->cws;
+    a.ws_bytes = kWorkspaceBytes;
+    return launch_tree_attn(a, be->cs);
+}
+
 static hipError_t run_mul_mat(wamx_backend * be, const wamx_tensor * node) {
+    if (is_mxfp4(node->src[0])) return run_mxfp4_mul_mat(be, node);
     return launch_gemm(mul_mat_args(be, node), be->cs);
 }
 
@@ -293,6 +420,7 @@ static GemmArgs linear_args(wamx_backend * be, const wamx_tensor * node) {
 }
 
 static hipError_t run_linear(wamx_backend * be, const wamx_tensor * node) {
+    if (is_mxfp4(node->src[0])) return run_mxfp4_linear(be, node);
     return launch_gemm(linear_args(be, node), be->cs);
 }
 
@@ -733,6 +861,7 @@ static hipError_t compute_node(wamx_backend * be, wamx_tensor * node) {
         case WAMX_OP_DUP:
         case WAMX_OP_CONT:
         case WAMX_OP_CPY:
+            if (is_mxfp4(s0) || is_mxfp4(node)) return run_mxfp4_copy(be, s0, node);
             return launch_copy(ref_of(s0), ref_of(node), s);
         case WAMX_OP_ADD:
             if (node->src[2]) {
@@ -789,6 +918,10 @@ static hipError_t compute_node(wamx_backend * be, wamx_tensor * node) {
                 return launch_bias_gelu_bf16(s0->data, s1->data, node->data, wamx_nelements(s0), s1->ne[0], s);
             return launch_unary(node->op_params[0], ref_of(s0), ref_of(node), 1.0f, 0.0f, s);
         case WAMX_OP_GET_ROWS:
+            if (is_mxfp4(s0))
+                return launch_mx_dequantize(s0->data, (int64_t) s0->nb[1], (const int32_t *) s1->data, s0->ne[1],
+                                            node->data, node->type, (int64_t) node->nb[1] / es(node), s1->ne[0],
+                                            s0->ne[0], s);
             return launch_get_rows(ref_of(s0), (const int32_t *) s1->data, ref_of(node), s);
         case WAMX_OP_IM2COL: {
             // ggml_im2col: kernel size from the kernel tensor, op_params {s0, s1, p0, p1, d0, d1, is_2D}.
@@ -826,6 +959,10 @@ static hipError_t compute_node(wamx_backend * be, wamx_tensor * node) {
         case WAMX_OP_EULER_STEP:
             return launch_euler_step(s0->data, s1->data, (const float *) node->src[2]->data, node->data,
                                      wamx_nelements(node), s);
+        case WAMX_OP_HEAD_NORM_ROPE:
+            return run_head_norm_rope(be, node);
+        case WAMX_OP_TREE_ATTN:
+            return run_tree_attn(be, node);
         case WAMX_OP_MLP_SMALL:
             return launch_mlp_small(s0->data, s1->data, node->src[2]->data, node->src[3]->data, node->src[4]->data,
                                     node->data, s0->ne[1], s0->ne[0], s1->ne[1], node->src[3]->ne[1],
@@ -884,6 +1021,14 @@ static bool supports(const wamx_tensor * t) {
         case WAMX_OP_DUP:
         case WAMX_OP_CONT:
         case WAMX_OP_CPY:
+            if (is_mxfp4(s0) || is_mxfp4(t)) {
+                // Quantise or dequantise rows of whole blocks, one shape.
+                const wamx_tensor * q = is_mxfp4(t) ? t : s0;
+                const wamx_tensor * v = is_mxfp4(t) ? s0 : t;
+                return t->op == WAMX_OP_CPY && float_type(v) && is_mxfp4(q) && wamx_are_same_shape(s0, t) &&
+                       rows_contig(s0) && rows_contig(t) && q->ne[0] % wamx_blck_size(q->type) == 0 &&
+                       v->nb[1] % es(v) == 0 && (q == s0 || wamx_is_contiguous(t));
+            }
             return ok_type(s0) && ok_type(t) && wamx_nelements(s0) == wamx_nelements(t);
         case WAMX_OP_ADD:
             if (t->src[2]) {  // gated residual bf16 (native-bf16.patch:594-612)
@@ -910,6 +1055,12 @@ static bool supports(const wamx_tensor * t) {
             return true;
         }
         case WAMX_OP_GET_ROWS:
+            if (is_mxfp4(s0))
+                return rows_contig(s0) && s0->ne[0] % wamx_blck_size(s0->type) == 0 && s0->ne[2] == 1 &&
+                       s0->ne[3] == 1 && s0->ne[1] > 0 && s1 && s1->type == WAMX_TYPE_I32 && rows_contig(s1) &&
+                       wamx_nelements(s1) == s1->ne[0] && float_type(t) && t->ne[0] == s0->ne[0] &&
+                       t->ne[1] == s1->ne[0] && t->ne[2] == 1 && t->ne[3] == 1 && rows_contig(t) &&
+                       t->nb[1] % es(t) == 0;
             return ok_type(s0) && s1 && s1->type == WAMX_TYPE_I32 && rows_contig(s1) && t->ne[0] == s0->ne[0] &&
                    t->ne[1] == s1->ne[0] && t->ne[2] == s1->ne[1] && float_type(t);
         case WAMX_OP_NORM:
@@ -938,6 +1089,11 @@ static bool supports(const wamx_tensor * t) {
                 (t->type != WAMX_TYPE_F32 && t->type != WAMX_TYPE_BF16))
                 return false;
             if (tensor_is_tiled(s0)) return tiled_product_ok(s1) && wamx_is_contiguous(t);
+            if (is_mxfp4(s0))
+                return s0->ne[0] > 0 && s0->ne[0] % wamx_blck_size(s0->type) == 0 && rows_contig(s0) &&
+                       (s1->type == WAMX_TYPE_BF16 || s1->type == WAMX_TYPE_F32) && rows_contig(s1) &&
+                       s1->nb[1] % es(s1) == 0 && s1->nb[2] % es(s1) == 0 && s1->nb[3] % es(s1) == 0 &&
+                       wamx_is_contiguous(t);
             return (s0->type == WAMX_TYPE_BF16 || s0->type == WAMX_TYPE_F32) &&
                    (s1->type == WAMX_TYPE_BF16 || s1->type == WAMX_TYPE_F32) && rows_contig(s0) && rows_contig(s1) &&
                    wamx_is_contiguous(t);
@@ -984,6 +1140,10 @@ static bool supports(const wamx_tensor * t) {
             return check_modulation(t) == nullptr;
         case WAMX_OP_EULER_STEP:
             return check_euler_step(t) == nullptr;
+        case WAMX_OP_HEAD_NORM_ROPE:
+            return check_head_norm_rope(t) == nullptr;
+        case WAMX_OP_TREE_ATTN:
+            return check_tree_attn(t) == nullptr;
         case WAMX_OP_MLP_SMALL:
             return check_mlp_small(t) == nullptr;
         default:
@@ -1137,7 +1297,9 @@ static wamx_status run_nodes(wamx_backend * be, wamx_cgraph * g) {
         int members[8] = {i};
         int nm = 1;
         bool fused = false;
-        if (node->op == WAMX_OP_LINEAR && be->fuse_rows) {
+        // A product with a weight in MXFP4 runs by itself.
+        const bool mx = (node->op == WAMX_OP_LINEAR || node->op == WAMX_OP_MUL_MAT) && is_mxfp4(node->src[0]);
+        if (node->op == WAMX_OP_LINEAR && be->fuse_rows && !mx) {
             RowPost post;
             const int last = match_row_post(g, i, n, post, two);
             if (last > i) {
@@ -1167,7 +1329,7 @@ static wamx_status run_nodes(wamx_backend * be, wamx_cgraph * g) {
                 }
             }
         }
-        if (node->op == WAMX_OP_MUL_MAT || node->op == WAMX_OP_CONV_2D) {
+        if ((node->op == WAMX_OP_MUL_MAT && !mx) || node->op == WAMX_OP_CONV_2D) {
             Chain c;
             const int last = match_chain(g, i, n, two, true, c);
             int dep = -1;
@@ -1950,6 +2112,180 @@ wamx_status wamx_op_joint_attn(wamx_backend_t be, const void * q, const void * k
     a.ws = be->workspace;
     a.ws_bytes = kWorkspaceBytes;
     WAMX_LAUNCH(launch_joint_attn(a, be->stream));
+}
+
+// The backend's device for the calls below, and the caller's again after them.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(wamx_backend_t be) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != be->dev->index) hipSetDevice(be->dev->index);
+        else before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) hipSetDevice(before);
+    }
+};
+
+wamx_status wamx_op_quantize_mxfp4(wamx_backend_t be, const void * x, int32_t x_type, int64_t ldx, void * q,
+                                   int64_t rows, int64_t cols) {
+    WAMX_REQUIRE(be && x && q, "wamx_op_quantize_mxfp4: null argument");
+    WAMX_REQUIRE(x_type == WAMX_TYPE_F32 || x_type == WAMX_TYPE_F16 || x_type == WAMX_TYPE_BF16,
+                 "wamx_op_quantize_mxfp4: x type");
+    WAMX_REQUIRE(rows >= 0 && cols > 0 && cols % 32 == 0 && ldx >= cols,
+                 "wamx_op_quantize_mxfp4: rows of whole 32-value blocks");
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_mx_quantize(x, x_type, ldx, q, rows, cols, be->stream));
+}
+
+wamx_status wamx_op_dequantize_mxfp4(wamx_backend_t be, const void * q, void * y, int32_t y_type, int64_t ldy,
+                                     int64_t rows, int64_t cols) {
+    WAMX_REQUIRE(be && q && y, "wamx_op_dequantize_mxfp4: null argument");
+    WAMX_REQUIRE(y_type == WAMX_TYPE_F32 || y_type == WAMX_TYPE_F16 || y_type == WAMX_TYPE_BF16,
+                 "wamx_op_dequantize_mxfp4: y type");
+    WAMX_REQUIRE(rows >= 0 && cols > 0 && cols % 32 == 0 && ldy >= cols,
+                 "wamx_op_dequantize_mxfp4: rows of whole 32-value blocks");
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_mx_dequantize(q, mx_row_bytes(cols), nullptr, 0, y, y_type, ldy, rows, cols, be->stream));
+}
+
+wamx_status wamx_op_mul_mat_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type, int64_t ldx,
+                                  void * y, int32_t y_type, int64_t ldy, int64_t M, int64_t N, int64_t K) {
+    WAMX_REQUIRE(be && w && x && y, "wamx_op_mul_mat_mxfp4: null argument");
+    WAMX_REQUIRE(x_type == WAMX_TYPE_F32 || x_type == WAMX_TYPE_BF16, "wamx_op_mul_mat_mxfp4: x type");
+    WAMX_REQUIRE(y_type == WAMX_TYPE_F32 || y_type == WAMX_TYPE_BF16, "wamx_op_mul_mat_mxfp4: y type");
+    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0 && ldx >= K && ldy >= M,
+                 "wamx_op_mul_mat_mxfp4: sizes (K a multiple of 32)");
+    MxArgs a;
+    a.w = w;
+    a.w_stride = mx_row_bytes(K);
+    a.x = x;
+    a.x_type = x_type;
+    a.ldx = ldx;
+    a.y = y;
+    a.y_type = y_type;
+    a.ldy = ldy;
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.ws = be->workspace;
+    a.ws_bytes = kWorkspaceBytes;
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_mx_product(a, be->stream));
+}
+
+wamx_status wamx_op_linear_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type, const void * bias,
+                                 int32_t epilogue, const void * residual, const float * gate, void * y, int64_t M,
+                                 int64_t N, int64_t K) {
+    WAMX_REQUIRE(be && w && x && y, "wamx_op_linear_mxfp4: null argument");
+    WAMX_REQUIRE(x_type == WAMX_TYPE_F32 || x_type == WAMX_TYPE_BF16, "wamx_op_linear_mxfp4: x type");
+    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0, "wamx_op_linear_mxfp4: sizes (K a multiple of 32)");
+    WAMX_REQUIRE(epilogue >= WAMX_EPI_NONE && epilogue <= WAMX_EPI_BIAS_RESIDUAL, "wamx_op_linear_mxfp4: epilogue");
+    WAMX_REQUIRE(epilogue == WAMX_EPI_NONE || bias, "wamx_op_linear_mxfp4: bias required");
+    WAMX_REQUIRE((epilogue != WAMX_EPI_BIAS_GATED && epilogue != WAMX_EPI_BIAS_RESIDUAL) || residual,
+                 "wamx_op_linear_mxfp4: residual required");
+    WAMX_REQUIRE(epilogue != WAMX_EPI_BIAS_GATED || gate, "wamx_op_linear_mxfp4: gate required");
+    MxArgs a;
+    a.w = w;
+    a.w_stride = mx_row_bytes(K);
+    a.x = x;
+    a.x_type = x_type;
+    a.ldx = K;
+    a.y = y;
+    a.ldy = M;
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.epi = epilogue;
+    a.bias = bias;
+    a.res = residual;
+    a.ldres = M;
+    a.gate = gate;
+    a.ws = be->workspace;
+    a.ws_bytes = kWorkspaceBytes;
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_mx_product(a, be->stream));
+}
+
+wamx_status wamx_op_qkv_head_norm_rope(wamx_backend_t be, const void * x, int64_t ldx, const void * wq, const void * wk,
+                                       const int32_t * pos, const int32_t * past, void * q, void * k, void * vt,
+                                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t tokens, int64_t batch,
+                                       int64_t capacity, int64_t vt_ld, int rope_mode, int n_dims, float eps,
+                                       float freq_base) {
+    WAMX_REQUIRE(be && x && (!q || wq) && (!k || wk), "wamx_op_qkv_head_norm_rope: null argument");
+    WAMX_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
+                 "wamx_op_qkv_head_norm_rope: head_dim must be 64, 128 or 256");
+    WAMX_REQUIRE(heads >= 0 && heads <= 65535 && kv_heads >= 0 && kv_heads <= 65535 && tokens >= 0 && batch >= 0 &&
+                     tokens <= 0x7fffffff && ldx >= (heads + kv_heads + (vt ? kv_heads : 0)) * head_dim,
+                 "wamx_op_qkv_head_norm_rope: sizes");
+    WAMX_REQUIRE((!k && !vt) || capacity >= tokens, "wamx_op_qkv_head_norm_rope: more tokens than the cache holds");
+    WAMX_REQUIRE(!vt || vt_ld >= capacity, "wamx_op_qkv_head_norm_rope: V^T rows shorter than the cache");
+    WAMX_REQUIRE(rope_mode == 0 || rope_mode == 2, "wamx_op_qkv_head_norm_rope: rope mode 0 or 2");
+    WAMX_REQUIRE(n_dims >= 0 && n_dims <= head_dim && n_dims % 16 == 0,
+                 "wamx_op_qkv_head_norm_rope: rotated dimensions are a multiple of 16 up to head_dim");
+    WAMX_REQUIRE(n_dims == 0 || pos || (!q && !k), "wamx_op_qkv_head_norm_rope: positions required");
+    WAMX_REQUIRE(eps >= 0.0f && freq_base > 0.0f, "wamx_op_qkv_head_norm_rope: eps or frequency base");
+    HeadNormArgs a;
+    a.x = x;
+    a.ldx = ldx;
+    a.wq = wq;
+    a.wk = wk;
+    a.pos = pos;
+    a.past = past;
+    a.q = heads ? q : nullptr;
+    a.k = kv_heads ? k : nullptr;
+    a.vt = kv_heads ? vt : nullptr;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.tokens = tokens;
+    a.batch = batch;
+    a.k_rows = capacity;
+    a.vt_ld = vt_ld;
+    a.k_col = heads * head_dim;
+    a.v_col = (heads + kv_heads) * head_dim;
+    a.rope_mode = rope_mode;
+    a.n_dims = n_dims;
+    a.eps = eps;
+    a.freq_base = freq_base;
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_head_norm_rope(a, be->stream));
+}
+
+wamx_status wamx_op_tree_attn(wamx_backend_t be, const void * q, const void * k, const void * vt,
+                              const int32_t * parents, const int32_t * past, void * out, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim, int64_t tokens, int64_t batch, int64_t capacity,
+                              int64_t vt_ld, float scale) {
+    WAMX_REQUIRE(be && q && k && vt && parents && out, "wamx_op_tree_attn: null argument");
+    WAMX_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
+                 "wamx_op_tree_attn: head_dim must be 64, 128 or 256");
+    WAMX_REQUIRE(tokens >= 0 && tokens <= 256 && batch >= 0 && capacity >= tokens && capacity > 0,
+                 "wamx_op_tree_attn: at most 256 drafted tokens, within the cache's slots");
+    WAMX_REQUIRE(heads > 0 && kv_heads > 0 && heads <= 65535 && heads % kv_heads == 0,
+                 "wamx_op_tree_attn: heads must be a multiple of kv_heads");
+    WAMX_REQUIRE(batch <= 65535 / kv_heads, "wamx_op_tree_attn: batch * kv_heads above 65535");
+    WAMX_REQUIRE(vt_ld >= capacity && vt_ld % 8 == 0, "wamx_op_tree_attn: V^T rows are a multiple of 8 slots");
+    WAMX_REQUIRE(((uintptr_t) q | (uintptr_t) k | (uintptr_t) vt) % 16 == 0 && (uintptr_t) out % 4 == 0,
+                 "wamx_op_tree_attn: q, k and V^T must be 16-byte aligned");
+    TreeArgs a;
+    a.q = q;
+    a.k = k;
+    a.vt = vt;
+    a.parents = parents;
+    a.past = past;
+    a.out = out;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.tq = tokens;
+    a.batch = batch;
+    a.capacity = capacity;
+    a.vt_ld = vt_ld;
+    a.scale = scale;
+    a.ws = be->workspace;
+    a.ws_bytes = kWorkspaceBytes;
+    OnDevice on(be);
+    WAMX_LAUNCH(launch_tree_attn(a, be->stream));
 }
 
 wamx_status wamx_op_soft_max_f32(wamx_backend_t be, const float * x, float * y, int64_t rows, int64_t cols, float scale) {

@@ -15,6 +15,8 @@ const char * last_error_cstr();
 const char * check_linear(const wamx_tensor * t);
 const char * check_qk_norm_rope(const wamx_tensor * t);
 const char * check_joint_attn(const wamx_tensor * t);
+const char * check_head_norm_rope(const wamx_tensor * t);
+const char * check_tree_attn(const wamx_tensor * t);
 const char * check_modulation(const wamx_tensor * t);
 const char * check_euler_step(const wamx_tensor * t);
 const char * check_mlp_small(const wamx_tensor * t);
@@ -143,6 +145,78 @@ struct Chain {
 // The product and its chain; hipErrorNotSupported, launching nothing, where
 // the product is neither gemm_row16's nor one that gemm_gen splits along K.
 hipError_t launch_gemm_chain(const GemmArgs & a, const Chain & c, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// MXFP4 (WAMX_TYPE_MXFP4): rows of 17-byte blocks of 32 values.
+// ---------------------------------------------------------------------------
+constexpr int64_t kMxBlockBytes = 17;
+constexpr int64_t mx_row_bytes(int64_t cols) { return cols / 32 * kMxBlockBytes; }
+// q[rows] packed one after another from x (f32, f16 or bf16, row stride ldx).
+hipError_t launch_mx_quantize(const void * x, int32_t x_type, int64_t ldx, void * q, int64_t rows, int64_t cols,
+                              hipStream_t s);
+// The values of `nrows` packed rows (byte stride qs) as f32, f16 or bf16; with
+// `rows`, of rows rows[0 .. nrows) out of qrows (an index outside: NaN).
+hipError_t launch_mx_dequantize(const void * q, int64_t qs, const int32_t * rows, int64_t qrows, void * y,
+                                int32_t y_type, int64_t ldy, int64_t nrows, int64_t cols, hipStream_t s);
+// y[n][m] = epilogue(sum_k w[m][k] bf16(x[n][k])), w in MXFP4, f32 accumulation.
+struct MxArgs {
+    const void * w = nullptr;
+    int64_t w_stride = 0;                    // bytes of a weight row
+    const void * x = nullptr;
+    int32_t x_type = WAMX_TYPE_BF16;
+    int64_t ldx = 0;
+    void * y = nullptr;
+    int32_t y_type = WAMX_TYPE_BF16;
+    int64_t ldy = 0;
+    int64_t M = 0, N = 0, K = 0;
+    int32_t epi = WAMX_EPI_NONE;
+    const void * bias = nullptr;
+    const void * res = nullptr;
+    int64_t ldres = 0;
+    const float * gate = nullptr;
+    void * ws = nullptr;
+    size_t ws_bytes = 0;
+};
+hipError_t launch_mx_product(const MxArgs & a, hipStream_t s);
+
+// Packed QKV rows x [batch * tokens][ldx] (heads * dh query, kv_heads * dh key,
+// kv_heads * dh value columns) to q [batch][heads][tokens][dh], keys in
+// k [batch][kv_heads][k_rows][dh] and values in vt [batch][kv_heads][dh][vt_ld]
+// at slots past[b] + t.  Null q, k or vt: that part is left out.
+struct HeadNormArgs {
+    const void * x = nullptr;
+    int64_t ldx = 0;
+    const void * wq = nullptr;
+    const void * wk = nullptr;
+    const int32_t * pos = nullptr;           // [batch * tokens]
+    const int32_t * past = nullptr;          // [batch], null: 0
+    void * q = nullptr;
+    void * k = nullptr;
+    void * vt = nullptr;
+    int64_t heads = 0, kv_heads = 0, head_dim = 0, tokens = 0, batch = 0, k_rows = 0, vt_ld = 0;
+    // Columns of x where each part starts.
+    int64_t q_col = 0, k_col = 0, v_col = 0;
+    int rope_mode = 0, n_dims = 0;
+    float eps = 0.0f, freq_base = 0.0f;
+};
+hipError_t launch_head_norm_rope(const HeadNormArgs & a, hipStream_t s);
+
+// Attention of a tree of drafted tokens over a cache: q [batch][heads][tq][dh],
+// k [batch][kv_heads][capacity][dh], vt [batch][kv_heads][dh][vt_ld],
+// parents [batch][tq], past [batch], out [batch][tq][heads * dh].
+struct TreeArgs {
+    const void * q = nullptr;
+    const void * k = nullptr;
+    const void * vt = nullptr;
+    const int32_t * parents = nullptr;
+    const int32_t * past = nullptr;
+    void * out = nullptr;
+    int64_t heads = 0, kv_heads = 0, head_dim = 0, tq = 0, batch = 0, capacity = 0, vt_ld = 0;
+    float scale = 1.0f;
+    void * ws = nullptr;
+    size_t ws_bytes = 0;
+};
+hipError_t launch_tree_attn(const TreeArgs & a, hipStream_t s);
 
 // ---------------------------------------------------------------------------
 // Row-wise norms (bf16 / f32), bias+GELU, gated residuals.

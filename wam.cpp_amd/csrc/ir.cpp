@@ -64,12 +64,18 @@ static wamx_tensor * new_tensor_impl(wamx_context * ctx, int32_t type, int n_dim
         set_errorf("wamx_new_tensor: unsupported type %d", type);
         return nullptr;
     }
+    const int64_t blck = wamx_blck_size(type);
+    if (blck > 1 && ne[0] % blck != 0) {
+        set_errorf("wamx_new_tensor: rows of %s are whole blocks of %lld values, not %lld", wamx_type_name(type),
+                   (long long) blck, (long long) ne[0]);
+        return nullptr;
+    }
     auto t = std::make_unique<wamx_tensor>();
     memset(t.get(), 0, sizeof(wamx_tensor));
     t->type = type;
     for (int i = 0; i < WAMX_MAX_DIMS; ++i) t->ne[i] = i < n_dims ? ne[i] : 1;
     t->nb[0] = wamx_type_size(type);
-    for (int i = 1; i < WAMX_MAX_DIMS; ++i) t->nb[i] = t->nb[i - 1] * (size_t)t->ne[i - 1];
+    for (int i = 1; i < WAMX_MAX_DIMS; ++i) t->nb[i] = t->nb[i - 1] * (size_t) (i == 1 ? t->ne[0] / blck : t->ne[i - 1]);
     t->op = WAMX_OP_NONE;
     t->lane = ctx->lane;
     wamx_tensor * raw = t.get();
@@ -112,9 +118,11 @@ static bool contig(const wamx_tensor * t) { return t && wamx_is_contiguous(t); }
 const char * check_linear(const wamx_tensor * t) {
     const wamx_tensor *w = t->src[0], *x = t->src[1], *bias = t->src[2], *res = t->src[3], *gate = t->src[4];
     const int32_t epi = t->op_params[0];
-    if (!is_bf16(w) || !x || (x->type != WAMX_TYPE_BF16 && x->type != WAMX_TYPE_F32)) return "types";
+    const bool mx = w && w->type == WAMX_TYPE_MXFP4;
+    if ((!is_bf16(w) && !mx) || !x || (x->type != WAMX_TYPE_BF16 && x->type != WAMX_TYPE_F32)) return "types";
     if (w->ne[0] != x->ne[0] || w->ne[2] != 1 || w->ne[3] != 1 || x->ne[2] != 1 || x->ne[3] != 1) return "shapes";
-    if (w->nb[0] != 2 || x->nb[0] != wamx_type_size(x->type)) return "rows must be contiguous";
+    if (w->nb[0] != wamx_type_size(w->type) || x->nb[0] != wamx_type_size(x->type)) return "rows must be contiguous";
+    if (mx && w->ne[0] % wamx_blck_size(w->type) != 0) return "rows of whole blocks";
     const int64_t M = w->ne[1], N = x->ne[1];
     if (epi < WAMX_EPI_NONE || epi > WAMX_EPI_BIAS_RESIDUAL) return "epilogue";
     if (epi != WAMX_EPI_NONE && (!is_bf16(bias) || bias->ne[0] != M || bias->nb[0] != 2)) return "bias";
@@ -218,6 +226,67 @@ const char * check_joint_attn(const wamx_tensor * t) {
             return "V^T layout";
     if (!is_bf16(t) || t->ne[0] != dh * H || t->ne[1] != Tq || t->ne[2] != B || t->ne[3] != 1 || !contig(t))
         return "output";
+    return nullptr;
+}
+
+static bool head_dim_ok(int64_t dh) { return dh == 64 || dh == 128 || dh == 256; }
+
+// x [dh * H, T * B] rows; dst [dh, rows, H, B] (queries and keys, contiguous)
+// or V^T [rows, dh, H, B] (op_params[4] = 1, rows of 8-value multiples).
+const char * check_head_norm_rope(const wamx_tensor * t) {
+    const wamx_tensor *x = t->src[0], *weight = t->src[1], *dst = t->src[2], *past = t->src[3], *pos = t->src[4];
+    const bool vt = t->op_params[4] != 0;
+    if (!is_bf16(x) || !is_bf16(dst) || !is_bf16(t) || (!vt && !is_bf16(weight))) return "types";
+    const int64_t dh = dst->ne[vt ? 1 : 0], rows = dst->ne[vt ? 0 : 1], H = dst->ne[2], B = dst->ne[3];
+    if (!head_dim_ok(dh)) return "head_dim must be 64, 128 or 256";
+    if (H < 1 || H > 65535 || B < 1 || x->ne[0] != dh * H || x->ne[1] % B != 0 || x->ne[2] != 1 || x->ne[3] != 1 ||
+        x->nb[0] != 2 || x->nb[1] % 2 != 0)
+        return "rows [head_dim * heads, tokens * sequences]";
+    const int64_t T = x->ne[1] / B;
+    if (T > rows) return "more tokens than the destination holds";
+    if (vt ? dst->nb[0] != 2 || dst->nb[1] % 2 != 0 || dst->nb[1] < (size_t) rows * 2 ||
+                 dst->nb[2] != dst->nb[1] * (size_t) dh || dst->nb[3] != dst->nb[2] * (size_t) H
+           : !contig(dst))
+        return "destination layout";
+    for (int i = 0; i < 4; ++i)
+        if (t->ne[i] != dst->ne[i] || t->nb[i] != dst->nb[i]) return "result must be the destination";
+    if (past && (past->type != WAMX_TYPE_I32 || wamx_nelements(past) != B || !contig(past)))
+        return "lengths: one i32 per sequence";
+    if (vt) return nullptr;
+    if (weight->ne[0] != dh || wamx_nelements(weight) != dh || weight->nb[0] != 2) return "norm weight [head_dim]";
+    const int mode = t->op_params[0], dims = t->op_params[1];
+    if (mode != 0 && mode != 2) return "rope mode 0 (neighbours) or 2 (halves)";
+    if (dims < 0 || dims > dh || dims % 16 != 0) return "rotated dimensions: a multiple of 16 up to head_dim";
+    float eps, base;
+    memcpy(&eps, &t->op_params[2], 4);
+    memcpy(&base, &t->op_params[3], 4);
+    if (!(eps >= 0.0f) || !(base > 0.0f)) return "eps or frequency base";
+    if (dims > 0 && (!pos || pos->type != WAMX_TYPE_I32 || wamx_nelements(pos) != T * B || !contig(pos)))
+        return "positions: one i32 per token";
+    return nullptr;
+}
+
+const char * check_tree_attn(const wamx_tensor * t) {
+    const wamx_tensor *q = t->src[0], *k = t->src[1], *v = t->src[2], *parents = t->src[3], *past = t->src[4];
+    if (!is_bf16(q) || !is_bf16(k) || !is_bf16(v) || !is_bf16(t)) return "types";
+    const int64_t dh = q->ne[0], T = q->ne[1], H = q->ne[2], B = q->ne[3], cap = k->ne[1], KV = k->ne[2];
+    if (!head_dim_ok(dh)) return "head_dim must be 64, 128 or 256";
+    if (T < 1 || T > 256 || cap < T) return "1 to 256 drafted tokens, at most the cache's slots";
+    if (H < 1 || KV < 1 || B < 1 || H % KV != 0 || B * KV > 65535) return "heads";
+    if (k->ne[0] != dh || k->ne[3] != B || v->ne[0] != cap || v->ne[1] != dh || v->ne[2] != KV || v->ne[3] != B)
+        return "cache shapes";
+    if (!contig(q) || !contig(k)) return "q and k must be contiguous";
+    if (v->nb[0] != 2 || v->nb[1] % 16 != 0 || v->nb[1] < (size_t) cap * 2 || v->nb[2] != v->nb[1] * (size_t) dh ||
+        v->nb[3] != v->nb[2] * (size_t) KV)
+        return "V^T layout";
+    if (!parents || parents->type != WAMX_TYPE_I32 || wamx_nelements(parents) != T * B || !contig(parents))
+        return "parents: one i32 per drafted token";
+    if (past && (past->type != WAMX_TYPE_I32 || wamx_nelements(past) != B || !contig(past)))
+        return "lengths: one i32 per sequence";
+    // Operands are read in 16-byte pieces.
+    for (const wamx_tensor * s : {q, k, v})
+        if ((uintptr_t) s->data % 16 != 0) return "q, k and V^T must be 16-byte aligned";
+    if (t->ne[0] != dh * H || t->ne[1] != T || t->ne[2] != B || t->ne[3] != 1 || !contig(t)) return "output";
     return nullptr;
 }
 
@@ -333,9 +402,12 @@ size_t wamx_type_size(int32_t type) {
         case WAMX_TYPE_F16: return 2;
         case WAMX_TYPE_BF16: return 2;
         case WAMX_TYPE_I32: return 4;
+        case WAMX_TYPE_MXFP4: return 17;
         default: return 0;
     }
 }
+
+int64_t wamx_blck_size(int32_t type) { return type == WAMX_TYPE_MXFP4 ? 32 : 1; }
 
 const char * wamx_type_name(int32_t type) {
     switch (type) {
@@ -343,6 +415,7 @@ const char * wamx_type_name(int32_t type) {
         case WAMX_TYPE_F16: return "f16";
         case WAMX_TYPE_BF16: return "bf16";
         case WAMX_TYPE_I32: return "i32";
+        case WAMX_TYPE_MXFP4: return "mxfp4";
         default: return "unknown";
     }
 }
@@ -352,7 +425,7 @@ const char * wamx_op_name(int32_t op) {
         "NONE", "DUP", "ADD", "MUL", "SCALE", "CPY", "CONT", "RESHAPE", "VIEW", "PERMUTE",
         "TRANSPOSE", "CONCAT", "REPEAT", "NORM", "RMS_NORM", "MUL_MAT", "SOFT_MAX", "ROPE",
         "UNARY", "GET_ROWS", "IM2COL", "CONV_2D", "LINEAR", "QK_NORM_ROPE", "JOINT_ATTN", "MODULATION",
-        "EULER_STEP", "MLP_SMALL",
+        "EULER_STEP", "MLP_SMALL", "HEAD_NORM_ROPE", "TREE_ATTN",
     };
     return (op >= 0 && op < WAMX_OP_COUNT) ? names[op] : "?";
 }
@@ -363,16 +436,20 @@ int64_t wamx_nrows(const wamx_tensor * t) { return t->ne[1] * t->ne[2] * t->ne[3
 size_t wamx_nbytes(const wamx_tensor * t) {
     // Span of memory touched: 1 element + sum of (ne-1)*nb over dims.
     if (wamx_nelements(t) == 0) return 0;
+    const int64_t blck = wamx_blck_size(t->type);
     size_t n = wamx_type_size(t->type);
-    for (int i = 0; i < WAMX_MAX_DIMS; ++i) n += (size_t)(t->ne[i] - 1) * t->nb[i];
+    n += (size_t) (t->ne[0] / blck - 1) * t->nb[0];
+    for (int i = 1; i < WAMX_MAX_DIMS; ++i) n += (size_t)(t->ne[i] - 1) * t->nb[i];
     return n;
 }
 
 bool wamx_is_contiguous(const wamx_tensor * t) {
+    const int64_t blck = wamx_blck_size(t->type);
     size_t expect = wamx_type_size(t->type);
     for (int i = 0; i < WAMX_MAX_DIMS; ++i) {
-        if (t->ne[i] != 1 && t->nb[i] != expect) return false;
-        expect *= (size_t)t->ne[i];
+        const int64_t ne = i == 0 ? t->ne[0] / blck : t->ne[i];
+        if (ne != 1 && t->nb[i] != expect) return false;
+        expect *= (size_t) ne;
     }
     return true;
 }
@@ -897,6 +974,54 @@ wamx_tensor * wamx_modulation(wamx_context * ctx, wamx_tensor * mod, wamx_tensor
     return checked(t, check_modulation, "wamx_modulation");
 }
 
+wamx_tensor * wamx_qk_head_norm_rope(wamx_context * ctx, wamx_tensor * x, wamx_tensor * weight, wamx_tensor * dst,
+                                     wamx_tensor * past, wamx_tensor * pos, int rope_mode, int n_dims, float eps,
+                                     float freq_base) {
+    if (!x || !weight || !dst) return fail("wamx_qk_head_norm_rope");
+    wamx_tensor * t = view_impl(ctx, dst, 4, dst->ne, 0);
+    if (!t) return nullptr;
+    memcpy(t->nb, dst->nb, sizeof t->nb);
+    t->op = WAMX_OP_HEAD_NORM_ROPE;
+    t->op_params[0] = rope_mode;
+    t->op_params[1] = n_dims;
+    set_param_f32(t, 2, eps);
+    set_param_f32(t, 3, freq_base);
+    t->src[0] = x;
+    t->src[1] = weight;
+    t->src[2] = dst;
+    t->src[3] = past;
+    t->src[4] = pos;
+    return checked(t, check_head_norm_rope, "wamx_qk_head_norm_rope");
+}
+
+wamx_tensor * wamx_vt_append(wamx_context * ctx, wamx_tensor * x, wamx_tensor * dst, wamx_tensor * past) {
+    if (!x || !dst) return fail("wamx_vt_append");
+    wamx_tensor * t = view_impl(ctx, dst, 4, dst->ne, 0);
+    if (!t) return nullptr;
+    memcpy(t->nb, dst->nb, sizeof t->nb);
+    t->op = WAMX_OP_HEAD_NORM_ROPE;
+    t->op_params[4] = 1;
+    t->src[0] = x;
+    t->src[2] = dst;
+    t->src[3] = past;
+    return checked(t, check_head_norm_rope, "wamx_vt_append");
+}
+
+wamx_tensor * wamx_tree_attn(wamx_context * ctx, wamx_tensor * q, wamx_tensor * k, wamx_tensor * v,
+                             wamx_tensor * parents, wamx_tensor * past, float scale) {
+    if (!q || !k || !v || !parents) return fail("wamx_tree_attn");
+    wamx_tensor * t = wamx_new_tensor_3d(ctx, WAMX_TYPE_BF16, q->ne[0] * q->ne[2], q->ne[1], q->ne[3]);
+    if (!t) return nullptr;
+    t->op = WAMX_OP_TREE_ATTN;
+    set_param_f32(t, 0, scale);
+    t->src[0] = q;
+    t->src[1] = k;
+    t->src[2] = v;
+    t->src[3] = parents;
+    t->src[4] = past;
+    return checked(t, check_tree_attn, "wamx_tree_attn");
+}
+
 wamx_tensor * wamx_euler_step(wamx_context * ctx, wamx_tensor * action, wamx_tensor * velocity, wamx_tensor * dt) {
     if (!action || !velocity || !dt) return fail("wamx_euler_step");
     wamx_tensor * t = new_tensor_impl(ctx, WAMX_TYPE_BF16, 4, action->ne);
@@ -1053,7 +1178,8 @@ static int32_t ggml_type_by_name(const char * name) {
     static const struct {
         const char * n;
         int32_t t;
-    } types[] = {{"f32", WAMX_TYPE_F32}, {"f16", WAMX_TYPE_F16}, {"bf16", WAMX_TYPE_BF16}, {"i32", WAMX_TYPE_I32}};
+    } types[] = {{"f32", WAMX_TYPE_F32}, {"f16", WAMX_TYPE_F16}, {"bf16", WAMX_TYPE_BF16}, {"i32", WAMX_TYPE_I32},
+                 {"mxfp4", WAMX_TYPE_MXFP4}};
     for (const auto & e : types)
         if (!strcmp(name, e.n)) return e.t;
     return -1;

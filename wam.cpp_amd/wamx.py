@@ -19,7 +19,7 @@ REPO = HERE.parent
 LIB_PATH = HERE / "libwamx.so"
 HEADER = REPO / "include" / "wamx" / "wamx.h"
 
-TYPE_F32, TYPE_F16, TYPE_I32, TYPE_BF16 = 0, 1, 26, 30
+TYPE_F32, TYPE_F16, TYPE_I32, TYPE_BF16, TYPE_MXFP4 = 0, 1, 26, 30, 39
 STATUS_SUCCESS = 0
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_GATED, EPI_BIAS_RESIDUAL = 0, 1, 2, 3, 4
 UNARY_GELU, UNARY_SILU, UNARY_GELU_ERF = 8, 10, 14
@@ -27,7 +27,7 @@ UNARY_GELU, UNARY_SILU, UNARY_GELU_ERF = 8, 10, 14
 OP_NAMES = ["NONE", "DUP", "ADD", "MUL", "SCALE", "CPY", "CONT", "RESHAPE", "VIEW", "PERMUTE",
             "TRANSPOSE", "CONCAT", "REPEAT", "NORM", "RMS_NORM", "MUL_MAT", "SOFT_MAX", "ROPE",
             "UNARY", "GET_ROWS", "IM2COL", "CONV_2D", "LINEAR", "QK_NORM_ROPE", "JOINT_ATTN", "MODULATION",
-            "EULER_STEP", "MLP_SMALL"]
+            "EULER_STEP", "MLP_SMALL", "HEAD_NORM_ROPE", "TREE_ATTN"]
 OP = {name: i for i, name in enumerate(OP_NAMES)}
 
 
@@ -136,6 +136,18 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
         "wamx_op_rope_table": (C.c_int, [vp, C.c_int, vp, vp, vp, i64, i64, f32, vp]),
         "wamx_op_qk_norm_rope_table": (C.c_int, [vp, vp, i64, vp, vp, i64, i64, i64, i64, i64, vp, f32]),
         "wamx_mlp_small": (TensorP, [vp, TensorP, TensorP, TensorP, TensorP, TensorP, i32]),
+        "wamx_blck_size": (i64, [i32]),
+        "wamx_op_quantize_mxfp4": (C.c_int, [vp, vp, i32, i64, vp, i64, i64]),
+        "wamx_op_dequantize_mxfp4": (C.c_int, [vp, vp, vp, i32, i64, i64, i64]),
+        "wamx_op_mul_mat_mxfp4": (C.c_int, [vp, vp, vp, i32, i64, vp, i32, i64, i64, i64, i64]),
+        "wamx_op_linear_mxfp4": (C.c_int, [vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, i64]),
+        "wamx_op_qkv_head_norm_rope": (C.c_int, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64,
+                                                 i64, C.c_int, C.c_int, f32, f32]),
+        "wamx_op_tree_attn": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, f32]),
+        "wamx_qk_head_norm_rope": (TensorP, [vp, TensorP, TensorP, TensorP, TensorP, TensorP, C.c_int, C.c_int, f32,
+                                             f32]),
+        "wamx_vt_append": (TensorP, [vp, TensorP, TensorP, TensorP]),
+        "wamx_tree_attn": (TensorP, [vp, TensorP, TensorP, TensorP, TensorP, TensorP, f32]),
         "wamx_op_soft_max_f32": (C.c_int, [vp, vp, vp, i64, i64, f32]),
         "wamx_fill_normal": (C.c_int, [vp, vp, i32, i64, C.c_uint64, f32, f32]),
         "wamx_timer_new": (vp, [vp]),
