@@ -190,6 +190,19 @@ def test_tree_capacity_far_above_the_lengths(wx, be, rng):
     tree_case(wx, be, rng, 4, 4, 4, 2, 64, [0, 1, 12000, 20], 12004, fill=0x7F80)
 
 
+@pytest.mark.parametrize("batch", [64, 65, 70])
+def test_tree_many_sequences(wx, be, rng, batch):
+    """Slots shared out by length up to 64 sequences, evenly above; some empty, some long."""
+    past = [0 if b % 7 == 0 else 3000 - 40 * b for b in range(batch)]
+    tree_case(wx, be, rng, batch, 2, 2, 1, 64, past, 3008, fill=0x7F80)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+def test_tree_zero_and_negative_scale(wx, be, rng, scale):
+    tree_case(wx, be, rng, 2, 5, 4, 2, 64, [100, 40], 120, scale=scale)
+    tree_case(wx, be, rng, 1, 40, 4, 2, 128, [100], 160, scale=scale)
+
+
 def test_tree_slots_without_a_token(wx, be, rng):
     """Padding sees nothing, gives zero rows, and nothing sees it."""
     par = [[-1, 0, -2, 1, 99, -5, 3], [-2] * 7]

@@ -2259,7 +2259,7 @@ wamx_status wamx_op_tree_attn(wamx_backend_t be, const void * q, const void * k,
     WAMX_REQUIRE(be && q && k && vt && parents && out, "wamx_op_tree_attn: null argument");
     WAMX_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
                  "wamx_op_tree_attn: head_dim must be 64, 128 or 256");
-    WAMX_REQUIRE(tokens >= 0 && tokens <= 256 && batch >= 0 && capacity >= tokens && capacity > 0,
+    WAMX_REQUIRE(tokens >= 0 && tokens <= 256 && batch >= 0 && capacity >= tokens && capacity > 0 && capacity <= 0x7fffffff,
                  "wamx_op_tree_attn: at most 256 drafted tokens, within the cache's slots");
     WAMX_REQUIRE(heads > 0 && kv_heads > 0 && heads <= 65535 && heads % kv_heads == 0,
                  "wamx_op_tree_attn: heads must be a multiple of kv_heads");

@@ -271,7 +271,7 @@ const char * check_tree_attn(const wamx_tensor * t) {
     if (!is_bf16(q) || !is_bf16(k) || !is_bf16(v) || !is_bf16(t)) return "types";
     const int64_t dh = q->ne[0], T = q->ne[1], H = q->ne[2], B = q->ne[3], cap = k->ne[1], KV = k->ne[2];
     if (!head_dim_ok(dh)) return "head_dim must be 64, 128 or 256";
-    if (T < 1 || T > 256 || cap < T) return "1 to 256 drafted tokens, at most the cache's slots";
+    if (T < 1 || T > 256 || cap < T || cap > 0x7fffffff) return "1 to 256 drafted tokens, at most the cache's slots";
     if (H < 1 || KV < 1 || B < 1 || H % KV != 0 || B * KV > 65535) return "heads";
     if (k->ne[0] != dh || k->ne[3] != B || v->ne[0] != cap || v->ne[1] != dh || v->ne[2] != KV || v->ne[3] != B)
         return "cache shapes";

@@ -4,18 +4,18 @@
 //   j over the cache slots [0, past) and the slots past + a of token i itself
 //   and its ancestors a (parents[]).
 //
-// K is [slot][dh] and V is held transposed, [dh][slot].  The cache bytes bound
-// it: every slot is read once, straight into matrix operands, by one pass that
-// carries each row's running maximum and sum.  S^T = K Q^T puts a query in a
-// lane's column and, with the slots of two 16-row tiles interleaved, eight
-// consecutive slots in its registers: exactly the operand of O^T = V^T P^T, so
-// the probabilities never leave the lane.  The rows are the drafted tokens of
-// every query head that shares a key head.  The slots are split over the waves
-// of a workgroup and over workgroups, whose f32 results a second launch joins.
+// K is [slot][dh] and V is held transposed, [dh][slot].  The cache's bytes bound
+// a few rows, the softmax's arithmetic and the products many; one pass over the
+// slots carries each row's running maximum and sum.  S^T = K Q^T puts a query
+// into a lane's column, the layout in which its probabilities are the operand
+// of O^T = V^T P^T.  The rows are the drafted tokens of every query head that
+// shares a key head, so the slots are read once for all of them.  The slots are
+// split over workgroups, whose f32 results a second launch joins.
 #include "../internal.h"
 #include "device.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace wamx {
 
@@ -26,11 +26,14 @@ struct TreeParams {
     const int32_t * parents;
     const int32_t * past;
     uint16_t * out;
-    float * po;          // [row][split][dh], or null: one split
-    float * pml;         // [row][split][2]
+    float * po;          // [unit][key head][row][dh], or null: nothing split
+    float * pml;         // [unit][key head][row][2]
     int64_t capacity, vt_ld;
-    int32_t heads, kv_heads, tq, splits;
-    float scale;         // times log2 e
+    int32_t heads, kv_heads, tq, batch;
+    int32_t even;        // units / batch for every sequence
+    int32_t units;       // parts of all sequences' slots, for each key head
+    float scale;         // times log2 e, positive
+    uint32_t q_and, q_xor;  // on pairs of Q's bits: the scale's sign, or 0
 };
 
 constexpr int kTreeWaves = 4, kTreeMax = 256, kTreeWords = kTreeMax / 32;
@@ -65,46 +68,173 @@ __device__ __forceinline__ const uint32_t (*tree_paths(TreePaths & s, const int3
 
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
-// NR tiles of 16 rows, slots in tiles of 32 HF.
-template <int DH, int NR, int HF>
-__global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_part(TreeParams p) {
-    constexpr int KC = DH / 32, DT = DH / 16, TILE = 32 * HF;
-    __shared__ TreePaths paths;
-    __shared__ __align__(16) f32x4_t red[kTreeWaves][DT * 64];
-    __shared__ float rm[kTreeWaves][NR][16], rl[kTreeWaves][NR][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c16 = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x;
-    const int64_t bz = blockIdx.z;
-    const int b = (int) (bz / p.kv_heads), hk = (int) (bz - (int64_t) b * p.kv_heads);
-    const int group = p.heads / p.kv_heads, rows = group * p.tq, row0 = blockIdx.y * 16 * NR;
-
-    // A length that does not fit leaves its sequence without keys.
-    const int64_t past = p.past ? p.past[b] : 0;
-    const int64_t n = past >= 0 && past + p.tq <= p.capacity ? past + p.tq : 0;
-    const int64_t tiles = (n + TILE - 1) / TILE;
-    const int64_t t0 = tiles * split / p.splits, t1 = tiles * (split + 1) / p.splits;
-    const int32_t * parents = p.parents + (int64_t) b * p.tq;
-    const uint32_t (*path)[kTreeWords] = paths.bits[0];
-    if (t1 * TILE > past) path = tree_paths(paths, parents, p.tq);
-
-    const uint16_t * kb = p.k + bz * p.capacity * DH;
-    const uint16_t * vb = p.vt + bz * DH * p.vt_ld;
-
-    // This lane's query of each row tile.
-    int tok[NR];
-    bool token[NR];
-    bf16x8_t qf[NR][KC];
+// Eight values of Q with the scale's sign.
+__device__ __forceinline__ bf16x8_t tree_q(const TreeParams & p, const uint16_t * q) {
+    union {
+        bf16x8_t v;
+        uint32_t w[4];
+    } u;
+    u.v = *(const bf16x8_t *) q;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const int row = min(row0 + i * 16 + c16, rows - 1);
-        tok[i] = row % p.tq;
-        const int pr = parents[tok[i]];
-        token[i] = pr >= -1 && pr < p.tq;
-        const uint16_t * qr = p.q + (((int64_t) b * p.heads + hk * group + row / p.tq) * p.tq + tok[i]) * DH;
+    for (int i = 0; i < 4; ++i) u.w[i] = (u.w[i] & p.q_and) ^ p.q_xor;
+    return u.v;
+}
+
+// 2^(scale q.k - m) of one row and slot, element by element: the weight of an
+// Inf or NaN value, which reaches its row whatever the weight's last bits.
+__device__ float tree_weight(const TreeParams & p, int64_t b, int64_t head, int64_t tok,
+                                                       const uint16_t * k, int dh, float m) {
+    const uint16_t * q = p.q + ((b * p.heads + head) * p.tq + tok) * dh;
+    float s = 0.0f;
+    for (int i = 0; i < dh; ++i)
+        s = fmaf(bf16_to_f32((uint16_t) ((q[i] & p.q_and) ^ p.q_xor)), bf16_to_f32(k[i]), s);
+    return __builtin_amdgcn_exp2f(s * p.scale - m);
+}
+
+// Eight values of V^T from `slot` on in a tile that reaches past `past`: slots
+// behind the last hold anything and become zero, and so do Inf and NaN of a
+// drafted slot, which must not reach the rows that do not see it (true: there
+// is one, added to the rows that do by itself).
+__device__ __forceinline__ bool tree_mask_values(uint32_t * w, int64_t slot, int64_t past, int64_t n) {
+    bool bad = false;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) qf[i][c] = *(const bf16x8_t *) (qr + c * 32 + g * 8);
+    for (int j = 0; j < 8; ++j) {
+        const bool odd = slot + j >= past && slot + j < n && not_finite_bf16(w[j >> 1] >> (16 * (j & 1)));
+        bad |= odd;
+        if (odd || slot + j >= n) w[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
     }
+    return bad;
+}
+
+// The units of the slots: sequence b gets 1 + (units - batch) tiles_b / tiles of
+// them (its share by length, but four tiles a unit at least), one after another;
+// units / batch each where the sequences are more than a wave's lanes (or the
+// product would pass 32 bits).  Unit u's sequence, the first of that sequence's
+// units and their number; no sequence (-1) past the last unit.
+constexpr int kTreeTile = 64;
+struct TreeUnit {
+    int b, first, count;
+};
+__device__ __forceinline__ int64_t tree_slots(const TreeParams & p, int b) {
+    // A length that does not fit leaves its sequence without slots.
+    const int64_t past = p.past ? p.past[b] : 0;
+    return past >= 0 && past + p.tq <= p.capacity ? past + p.tq : 0;
+}
+__device__ __forceinline__ TreeUnit tree_unit(const TreeParams & p, int u, int b_known = -1) {
+    if (p.even) {
+        const int each = (int) ((uint32_t) p.units / (uint32_t) p.batch);
+        const int b = b_known >= 0 ? b_known : (int) ((uint32_t) u / (uint32_t) each);
+        return {b < p.batch ? b : -1, b * each, each};
+    }
+    const int lane = threadIdx.x & 63;
+    const uint32_t tiles = lane < p.batch ? (uint32_t) ((tree_slots(p, lane) + kTreeTile - 1) / kTreeTile) : 0;
+    uint32_t sum = tiles;
+    for (int o = 1; o < p.batch; o <<= 1) sum += (uint32_t) __shfl_xor((int) sum, o);
+    // Past the batch's power of two the lanes hold nothing, and take nothing.
+    int mine = 0;
+    if (lane < p.batch) {
+        mine = 1 + (sum ? (int) ((uint32_t) (p.units - p.batch) * tiles / sum) : 0);
+        mine = min(mine, max(1, (int) (tiles / 4)));
+    }
+    int end = mine;  // inclusive prefix
+    for (int o = 1; o < p.batch; o <<= 1) {
+        const int v = __shfl_up(end, o);
+        if (lane >= o) end += v;
+    }
+    int b = b_known;
+    if (b < 0) {
+        const unsigned long long past_u = __ballot(lane < p.batch && end > u);
+        if (!past_u) return {-1, 0, 0};
+        b = __ffsll(past_u) - 1;
+    }
+    const int count = __shfl(mine, b);
+    return {b, __shfl(end, b) - count, count};
+}
+// The tiles [t0, t1) of part i out of `count`.
+__device__ __forceinline__ void tree_range(int64_t n, int i, int count, int64_t & t0, int64_t & t1) {
+    const uint32_t tiles = (uint32_t) ((n + kTreeTile - 1) / kTreeTile);
+    const uint32_t q = tiles / (uint32_t) count, r = tiles - q * (uint32_t) count;
+    t0 = q * (uint32_t) i + min((uint32_t) i, r);
+    t1 = t0 + q + ((uint32_t) i < r);
+}
+
+// A barrier that waits for this wave's LDS accesses alone: loads into registers
+// stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// NR tiles of 16 rows for a workgroup, slots in tiles of 64: wave w takes slots
+// 16w .. of a tile for the scores of all rows, and DH / 4 of the result's
+// dimensions for all rows and slots, so every K and V element is loaded once,
+// by one wave, into the registers that feed its matrix operand.  The rows (Q)
+// and the probabilities lie in LDS.  K of the next tile is requested when this
+// tile's scores are done and V when its product is.
+template <int DH, int NR>
+__global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) {
+    constexpr int KC = DH / 32, DT = DH / 64, TILE = 64, R = NR * 16, QCH = DH / 8;
+    __shared__ __align__(16) uint16_t qs[R * DH];
+    __shared__ __align__(16) uint16_t ps[R * TILE];
+    __shared__ float sm[kTreeWaves][R];
+    __shared__ TreePaths paths;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    const int group = p.heads / p.kv_heads, rows = group * p.tq;
+    // Row tiles of one unit are eight workgroups apart: the same XCD, whose L2
+    // then holds the slots they share.
+    const int rt = (rows + R - 1) / R;
+    const uint32_t id = blockIdx.x, at8 = id / (uint32_t) (8 * rt) * 8 + id % 8;
+    const int row0 = (int) (id / 8 % (uint32_t) rt) * R;
+    const int hk = (int) (at8 / (uint32_t) p.units), u = (int) at8 - hk * p.units;
+    if (hk >= p.kv_heads) return;
+    const TreeUnit unit = tree_unit(p, u);
+    if (unit.b < 0) return;
+    const int b = unit.b;
+    const int64_t n = tree_slots(p, b), past = n ? n - p.tq : 0;
+    int64_t t0, t1;
+    tree_range(n, u - unit.first, unit.count, t0, t1);
+    const int64_t bz = (int64_t) b * p.kv_heads + hk;
+    const int32_t * parents = p.parents + (int64_t) b * p.tq;
+
+    const uint16_t * kb = p.k + bz * p.capacity * DH + g * 8;
+    const uint16_t * vb = p.vt + (bz * DH + wave * (DH / 4) + c16) * p.vt_ld;
+    bf16x8_t kf[KC], vf[2][DT];
+    auto load_k = [&](int64_t kt) {
+        const int64_t slot = min(kt * TILE + wave * 16 + c16, n - 1);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kf[c] = *(const bf16x8_t *) (kb + slot * DH + c * 32);
+    };
+    auto load_v = [&](int64_t kt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t v0 = min(kt * TILE + h * 32 + g * 8, p.vt_ld - 8);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vf[h][d] = *(const bf16x8_t *) (vb + (int64_t) d * 16 * p.vt_ld + v0);
+        }
+    };
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+    }
+
+    // Q into LDS: 16-byte chunk c of row r at c ^ (r's swizzle), so that the 16
+    // rows of an operand read lie in different banks.
+    auto qswz = [](int r) { return DH == 64 ? (r >> 1) & 7 : r & 15; };
+    for (int e = threadIdx.x; e < R * QCH; e += kTreeWaves * 64) {
+        const int r = e / QCH, c = e % QCH, row = min(row0 + r, rows - 1);
+        const uint16_t * qr = p.q + (((int64_t) b * p.heads + hk * group + row / p.tq) * p.tq + row % p.tq) * DH;
+        *(bf16x8_t *) (qs + r * DH + (c ^ qswz(r)) * 8) = tree_q(p, qr + c * 8);
+    }
+    int tok[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) tok[i] = min(row0 + i * 16 + c16, rows - 1) % p.tq;
+    const uint32_t (*path)[kTreeWords] = paths.bits[0];
+    if (t0 < t1 && t1 * TILE > past) path = tree_paths(paths, parents, p.tq);
+    __syncthreads();
+
     float m[NR], l[NR];
     f32x4_t o[NR][DT];
 #pragma unroll
@@ -114,257 +244,469 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_part(TreeParams p) 
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0, 0, 0, 0};
     }
-
-    for (int64_t kt = t0 + wave; kt < t1; kt += kTreeWaves) {
+    bool bad = false;
+    for (int64_t kt = t0; kt < t1; ++kt) {
         const int64_t base = kt * TILE;
-        f32x4_t s[NR][2 * HF];
+        const bool edge = base + TILE > past;
+        f32x4_t s[NR];
 #pragma unroll
-        for (int u = 0; u < 2 * HF; ++u) {
-            // Row a of tile u is slot 8 (a / 4) + 4 (u % 2) + a % 4 of its half.
-            const int64_t slot = min(base + (u >> 1) * 32 + 8 * (c16 >> 2) + 4 * (u & 1) + (c16 & 3), n - 1);
-            bf16x8_t kf[KC];
+        for (int i = 0; i < NR; ++i) s[i] = (f32x4_t){0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < KC; ++c) kf[c] = *(const bf16x8_t *) (kb + slot * DH + c * 32 + g * 8);
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                s[i][u] = (f32x4_t){0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < KC; ++c)
-                    s[i][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], qf[i][c], s[i][u], 0, 0, 0);
+                const int r = i * 16 + c16;
+                const bf16x8_t q = *(const bf16x8_t *) (qs + r * DH + ((c * 4 + g) ^ qswz(r)) * 8);
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[c], q, s[i], 0, 0, 0);
             }
-        }
-        const bool edge = base + TILE > past;  // drafted slots, or the end, in this tile
-        bf16x8_t pf[NR][HF];
+        if (kt + 1 < t1) load_k(kt + 1);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 2 * HF; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = s[i][u][r] * p.scale;
-                    if (edge) {
-                        const int64_t slot = base + (u >> 1) * 32 + 8 * g + 4 * (u & 1) + r;
-                        bool seen = slot < past;
-                        if (slot >= past && slot < n) {
-                            const int a = (int) (slot - past);
-                            seen = path[tok[i]][a >> 5] >> (a & 31) & 1;
-                        }
-                        v = seen ? v : -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+                float v = s[i][r];
+                if (edge) {
+                    const int64_t slot = base + wave * 16 + 4 * g + r;
+                    bool seen = slot < past;
+                    if (slot >= past && slot < n) {
+                        const int a = (int) (slot - past);
+                        seen = path[tok[i]][a >> 5] >> (a & 31) & 1;
                     }
-                    s[i][u][r] = v;
-                    top = fmaxf(top, v);
+                    v = seen ? v : -INFINITY;
                 }
-            top = max_xor32(max_xor16(top));
-            const float mn = fmaxf(m[i], top);
-            const float base_m = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[i] - base_m);
-            float sum = 0.0f;
+                s[i][r] = v;
+                top = fmaxf(top, v);
+            }
+            top = max_xor32(max_xor16(top)) * p.scale;
+            if (g == 0) sm[wave][i * 16 + c16] = top;
+        }
+        lds_barrier();
 #pragma unroll
-            for (int u = 0; u < 2 * HF; ++u)
+        for (int i = 0; i < NR; ++i) {
+            const int r = i * 16 + c16;
+            const float mn = fmaxf(fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])), m[i]);
+            const float bm = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[i] - bm);
+            float pr[4], sum = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[i][u][r] = __builtin_amdgcn_exp2f(s[i][u][r] - base_m);
-                    sum += s[i][u][r];
-                }
+            for (int e = 0; e < 4; ++e) {
+                pr[e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.scale, -bm));
+                sum += pr[e];
+            }
             l[i] = l[i] * alpha + sum;
             if (__any(mn != m[i])) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[i][d] *= alpha;
             }
             m[i] = mn;
-#pragma unroll
-            for (int h = 0; h < HF; ++h) {
-                union {
-                    uint32_t d[4];
-                    bf16x8_t v;
-                } pk;
-                pk.d[0] = pack_bf16x2(s[i][2 * h][0], s[i][2 * h][1]);
-                pk.d[1] = pack_bf16x2(s[i][2 * h][2], s[i][2 * h][3]);
-                pk.d[2] = pack_bf16x2(s[i][2 * h + 1][0], s[i][2 * h + 1][1]);
-                pk.d[3] = pack_bf16x2(s[i][2 * h + 1][2], s[i][2 * h + 1][3]);
-                pf[i][h] = pk.v;
-            }
+            uint2 w;
+            w.x = pack_bf16x2(pr[0], pr[1]);
+            w.y = pack_bf16x2(pr[2], pr[3]);
+            *(uint2 *) (ps + r * TILE + ((2 * wave + (g >> 1)) ^ ((r >> 1) & 7)) * 8 + (g & 1) * 4) = w;
         }
-        bool bad = false;
+        lds_barrier();
+        if (edge) {
 #pragma unroll
-        for (int h = 0; h < HF; ++h) {
-            const int64_t v0 = base + h * 32 + g * 8;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                union {
-                    uint32_t w[4];
-                    bf16x8_t v;
-                } vf;
-                vf.v = (bf16x8_t){};
-                if (v0 < p.vt_ld) vf.v = *(const bf16x8_t *) (vb + (int64_t) (d * 16 + c16) * p.vt_ld + v0);
-                if (edge) {
-                    // Slots behind the last hold anything; a drafted slot's
-                    // values must not reach the rows that do not see it, which
-                    // for Inf and NaN takes the path below.
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t e = vf.w[j >> 1] >> (16 * (j & 1));
-                        const bool drafted = v0 + j >= past;
-                        const bool odd = drafted && v0 + j < n && not_finite_bf16(e);
-                        bad |= odd;
-                        if (odd || v0 + j >= n) vf.w[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-                    }
+                for (int d = 0; d < DT; ++d) {
+                    union {
+                        bf16x8_t v;
+                        uint32_t w[4];
+                    } u;
+                    u.v = vf[h][d];
+                    bad |= tree_mask_values(u.w, base + h * 32 + g * 8, past, n);
+                    vf[h][d] = u.v;
                 }
-#pragma unroll
-                for (int i = 0; i < NR; ++i)
-                    o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[i][h], o[i][d], 0, 0, 0);
-            }
         }
-        if (edge && __any(bad)) {
-            // Inf or NaN among the drafted values: added element by element to
-            // the rows whose path holds the slot.
-            float * pl = (float *) red[wave];  // [TILE][16], this wave's own
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
+                const int r = i * 16 + c16;
+                const bf16x8_t pf = *(const bf16x8_t *) (ps + r * TILE + ((4 * h + g) ^ ((r >> 1) & 7)) * 8);
 #pragma unroll
-                for (int u = 0; u < 2 * HF; ++u)
+                for (int d = 0; d < DT; ++d)
+                    o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[h][d], pf, o[i][d], 0, 0, 0);
+            }
+        if (kt + 1 < t1) load_v(kt + 1);
+    }
+    if (__any(bad)) {
+        // Inf or NaN among the drafted values: added element by element to the
+        // rows whose path holds the slot.
+        for (int64_t slot = max(t0 * TILE, past); slot < min(t1 * TILE, n); ++slot) {
+            const int a = (int) (slot - past);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) pl[((u >> 1) * 32 + 8 * g + 4 * (u & 1) + r) * 16 + c16] = s[i][u][r];
-                __builtin_amdgcn_wave_barrier();
-                for (int64_t slot = max(base, past); slot < min(base + TILE, n); ++slot) {
-                    const int a = (int) (slot - past);
-                    if (!(path[tok[i]][a >> 5] >> (a & 31) & 1)) continue;
-                    const float pr = pl[(int) (slot - base) * 16 + c16];
+            for (int i = 0; i < NR; ++i) {
+                if (!(path[tok[i]][a >> 5] >> (a & 31) & 1)) continue;
+                const int row = min(row0 + i * 16 + c16, rows - 1);
+                const float pr =
+                    tree_weight(p, b, hk * group + row / p.tq, tok[i], kb - g * 8 + slot * DH, DH, m[i]);
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t e = vb[(int64_t) (d * 16 + 4 * g + r) * p.vt_ld + slot];
-                            if (not_finite_bf16(e)) o[i][d][r] += pr * bf16_to_f32((uint16_t) e);
-                        }
-                }
-                __builtin_amdgcn_wave_barrier();
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t v = vb[(int64_t) (d * 16 + 4 * g + e - c16) * p.vt_ld + slot];
+                        if (not_finite_bf16(v)) o[i][d][e] += pr * bf16_to_f32(v);
+                    }
             }
         }
     }
 
-    // The waves' results, joined in wave order.
+    // The rows' sums over the lanes and waves that hold their parts.
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        l[i] = sum_xor32(sum_xor16(l[i]));
-        if (g == 0) {
-            rm[wave][i][c16] = m[i];
-            rl[wave][i][c16] = l[i];
-        }
+        const float t = sum_xor32(sum_xor16(l[i]));
+        if (g == 0) sm[wave][i * 16 + c16] = t;
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        float top = -INFINITY;
+        const int r = i * 16 + c16, row = row0 + r;
+        const float sum = (sm[0][r] + sm[1][r]) + (sm[2][r] + sm[3][r]);
+        if (row >= rows) continue;
+        const int pr = parents[tok[i]];
+        const bool none = !(pr >= -1 && pr < p.tq) || (sum == 0.0f && m[i] == -INFINITY);
+        const int d0 = wave * (DH / 4) + 4 * g;
+        if (p.po) {
+            const int64_t at = ((int64_t) u * p.kv_heads + hk) * rows + row;
 #pragma unroll
-        for (int w = 0; w < kTreeWaves; ++w) top = fmaxf(top, rm[w][i][c16]);
-        const float base_m = top == -INFINITY ? 0.0f : top;
-        const float f = __builtin_amdgcn_exp2f(m[i] - base_m);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) red[wave][d * 64 + lane] = o[i][d] * f;
-        __syncthreads();
-        for (int e = threadIdx.x; e < DT * 64; e += kTreeWaves * 64) {
-            const int q = e & 15, d = (e >> 6) * 16 + ((e >> 4) & 3) * 4;
-            const int row = row0 + i * 16 + q;
-            float big = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kTreeWaves; ++w) big = fmaxf(big, rm[w][i][q]);
-            const float bm = big == -INFINITY ? 0.0f : big;
-            f32x4_t v = red[0][e];
-            sum = rl[0][i][q] * __builtin_amdgcn_exp2f(rm[0][i][q] - bm);
-#pragma unroll
-            for (int w = 1; w < kTreeWaves; ++w) {
-                v += red[w][e];
-                sum += rl[w][i][q] * __builtin_amdgcn_exp2f(rm[w][i][q] - bm);
+            for (int d = 0; d < DT; ++d) *(f32x4_t *) (p.po + at * DH + d0 + d * 16) = o[i][d];
+            if (wave == 0 && g == 0) {
+                // A sum that is NaN must outlive a maximum that no score raised.
+                p.pml[2 * at] = none ? -INFINITY : m[i] == -INFINITY ? 0.0f : m[i];
+                p.pml[2 * at + 1] = none ? 0.0f : sum;
             }
-            if (row >= rows) continue;
-            const int t = row % p.tq;
-            const int pr = parents[t];
-            const bool has = pr >= -1 && pr < p.tq;
-            if (p.po) {
-                const int64_t at = (bz * rows + row) * p.splits + split;
-                *(f32x4_t *) (p.po + at * DH + d) = v;
-                if (d == 0) {
-                    p.pml[2 * at] = has ? big : -INFINITY;
-                    p.pml[2 * at + 1] = has ? sum : 0.0f;
-                }
-            } else {
-                const float inv = 1.0f / sum;
-                const bool none = !has || (sum == 0.0f && big == -INFINITY);
-                uint32_t w[2];
+        } else {
+            const float inv = none ? 0.0f : 1.0f / sum;
+            uint16_t * y = p.out + (((int64_t) b * p.tq + tok[i]) * p.heads + hk * group + row / p.tq) * DH + d0;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) w[r] = none ? 0u : pack_bf16x2(v[2 * r] * inv, v[2 * r + 1] * inv);
-                uint16_t * y = p.out + (((int64_t) b * p.tq + t) * p.heads + hk * group + row / p.tq) * DH + d;
-                *(uint32_t *) y = w[0];
-                *(uint32_t *) (y + 2) = w[1];
+            for (int d = 0; d < DT; ++d) {
+                *(uint32_t *) (y + d * 16) = none ? 0u : pack_bf16x2(o[i][d][0] * inv, o[i][d][1] * inv);
+                *(uint32_t *) (y + d * 16 + 2) = none ? 0u : pack_bf16x2(o[i][d][2] * inv, o[i][d][3] * inv);
             }
         }
-        __syncthreads();
     }
 }
 
-// out = sum_s po_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), splits in order: a wave
-// per row, DH / 64 values a lane.
-template <int DH>
-__global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int64_t total) {
-    const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= total) return;
+// Many rows: W waves of NR tiles of 16 rows each, every wave over all slots of
+// a tile, so a row's maximum, sum and probabilities stay in its wave.  S^T =
+// K Q^T puts a query in a lane's column, and with the slots of two 16-row tiles
+// interleaved (row a of tile u is slot 8 (a / 4) + 4 (u % 2) + a % 4 of its
+// half) eight consecutive slots in its registers: the operand of O^T = V^T P^T
+// as it stands.  K and V^T tiles of 64 slots go through registers into one of
+// two LDS buffers while the other is used; one barrier a tile.
+template <int DH, int NR, int W>
+__global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
+    constexpr int KC = DH / 32, DT = DH / 16, TILE = 64, R = W * NR * 16, QCH = DH / 8;
+    constexpr int KN = TILE * QCH / (W * 64), VN = DH * 8 / (W * 64);  // 16-byte pieces of a thread
+    __shared__ __align__(16) uint16_t kt_lds[2][TILE * DH];
+    __shared__ __align__(16) uint16_t vt_lds[2][DH * TILE];
+    __shared__ TreePaths paths;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
-    const int64_t bz = at / rows;
-    const int row = (int) (at - bz * rows);
-    const int64_t b = bz / p.kv_heads;
-    const int hk = (int) (bz - b * p.kv_heads);
-    const float * ml = p.pml + at * p.splits * 2;
-    float m = -INFINITY;
-    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ml[2 * s]);
-    m = wave_max(m);
-    constexpr int V = DH / 64;
-    float acc[V] = {}, sum = 0.0f;
-    const float * po = p.po + at * p.splits * DH + lane * V;
-    if (m != -INFINITY) {
-        for (int s = 0; s < p.splits; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-            sum += ml[2 * s + 1] * f;
+    const int rt = (rows + R - 1) / R;
+    const uint32_t id = blockIdx.x, at8 = id / (uint32_t) (8 * rt) * 8 + id % 8;
+    const int row0 = (int) (id / 8 % (uint32_t) rt) * R + wave * NR * 16;
+    const int hk = (int) (at8 / (uint32_t) p.units), u = (int) at8 - hk * p.units;
+    if (hk >= p.kv_heads) return;
+    const TreeUnit unit = tree_unit(p, u);
+    if (unit.b < 0) return;
+    const int b = unit.b;
+    const int64_t n = tree_slots(p, b), past = n ? n - p.tq : 0;
+    int64_t t0, t1;
+    tree_range(n, u - unit.first, unit.count, t0, t1);
+    const int64_t bz = (int64_t) b * p.kv_heads + hk;
+    const int32_t * parents = p.parents + (int64_t) b * p.tq;
+    const uint16_t * kb = p.k + bz * p.capacity * DH;
+    const uint16_t * vb = p.vt + bz * DH * p.vt_ld;
+
+    // 16 rows of an operand read fall into different banks: chunk c of K slot
+    // k at c ^ kswz(k) (the 16 slots of a tile differ in bits 0, 1, 3 and 4),
+    // of V^T row d at c ^ (d / 2) % 8.
+    auto kswz = [](int k) {
+        return DH == 64 ? ((k >> 1) & 1) | ((k >> 3) & 3) << 1 : (k & 3) | ((k >> 3) & 3) << 2;
+    };
+    bf16x8_t kr[KN], vr[VN];
+    auto request = [&](int64_t kt) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] += po[(int64_t) s * DH + v] * f;
+        for (int j = 0; j < KN; ++j) {
+            const int e = threadIdx.x + j * W * 64;
+            kr[j] = *(const bf16x8_t *) (kb + min(kt * TILE + e / QCH, n - 1) * DH + e % QCH * 8);
+        }
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+            const int e = threadIdx.x + j * W * 64;
+            vr[j] = *(const bf16x8_t *) (vb + (int64_t) (e >> 3) * p.vt_ld + min(kt * TILE + (e & 7) * 8, p.vt_ld - 8));
+        }
+    };
+    auto deposit = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < KN; ++j) {
+            const int e = threadIdx.x + j * W * 64, k = e / QCH;
+            *(bf16x8_t *) (kt_lds[buf] + k * DH + ((e % QCH) ^ kswz(k)) * 8) = kr[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+            const int e = threadIdx.x + j * W * 64, d = e >> 3;
+            *(bf16x8_t *) (vt_lds[buf] + d * TILE + ((e & 7) ^ ((d >> 1) & 7)) * 8) = vr[j];
+        }
+    };
+    if (t0 < t1) request(t0);
+    int tok[NR];
+    bf16x8_t qf[NR][KC];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int row = min(row0 + i * 16 + c16, rows - 1);
+        tok[i] = row % p.tq;
+        const uint16_t * qr = p.q + (((int64_t) b * p.heads + hk * group + row / p.tq) * p.tq + tok[i]) * DH;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) qf[i][c] = tree_q(p, qr + c * 32 + g * 8);
+    }
+    const uint32_t (*path)[kTreeWords] = paths.bits[0];
+    if (t0 < t1 && t1 * TILE > past) path = tree_paths(paths, parents, p.tq);
+    if (t0 < t1) deposit(0);
+    __syncthreads();
+
+    float m[NR], l[NR];
+    f32x4_t o[NR][DT];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0, 0, 0, 0};
+    }
+    bool bad = false;
+    for (int64_t kt = t0; kt < t1; ++kt) {
+        const int buf = (int) (kt - t0) & 1;
+        const int64_t base = kt * TILE;
+        const bool edge = base + TILE > past;
+        if (kt + 1 < t1) request(kt + 1);
+        if (row0 < rows) {
+            f32x4_t s[NR][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = (u >> 1) * 32 + 8 * (c16 >> 2) + 4 * (u & 1) + (c16 & 3);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) s[i][u] = (f32x4_t){0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const bf16x8_t kf = *(const bf16x8_t *) (kt_lds[buf] + k * DH + ((c * 4 + g) ^ kswz(k)) * 8);
+#pragma unroll
+                    for (int i = 0; i < NR; ++i)
+                        s[i][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][c], s[i][u], 0, 0, 0);
+                }
+            }
+            bf16x8_t pf[NR][2];
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float v = s[i][u][r];
+                        if (edge) {
+                            const int64_t slot = base + (u >> 1) * 32 + 8 * g + 4 * (u & 1) + r;
+                            bool seen = slot < past;
+                            if (slot >= past && slot < n) {
+                                const int a = (int) (slot - past);
+                                seen = path[tok[i]][a >> 5] >> (a & 31) & 1;
+                            }
+                            v = seen ? v : -INFINITY;
+                        }
+                        s[i][u][r] = v;
+                        top = fmaxf(top, v);
+                    }
+                top = max_xor32(max_xor16(top)) * p.scale;
+                const float mn = fmaxf(m[i], top);
+                const float bm = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[i] - bm);
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[i][u][r] = __builtin_amdgcn_exp2f(fmaf(s[i][u][r], p.scale, -bm));
+                        sum += s[i][u][r];
+                    }
+                l[i] = l[i] * alpha + sum;
+                if (__any(mn != m[i])) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[i][d] *= alpha;
+                }
+                m[i] = mn;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    union {
+                        uint32_t d[4];
+                        bf16x8_t v;
+                    } pk;
+                    pk.d[0] = pack_bf16x2(s[i][2 * h][0], s[i][2 * h][1]);
+                    pk.d[1] = pack_bf16x2(s[i][2 * h][2], s[i][2 * h][3]);
+                    pk.d[2] = pack_bf16x2(s[i][2 * h + 1][0], s[i][2 * h + 1][1]);
+                    pk.d[3] = pack_bf16x2(s[i][2 * h + 1][2], s[i][2 * h + 1][3]);
+                    pf[i][h] = pk.v;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int dr = d * 16 + c16;
+                    union {
+                        bf16x8_t v;
+                        uint32_t w[4];
+                    } u;
+                    u.v = *(const bf16x8_t *) (vt_lds[buf] + dr * TILE + ((4 * h + g) ^ ((dr >> 1) & 7)) * 8);
+                    if (edge) bad |= tree_mask_values(u.w, base + h * 32 + g * 8, past, n);
+#pragma unroll
+                    for (int i = 0; i < NR; ++i)
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, pf[i][h], o[i][d], 0, 0, 0);
+                }
+        }
+        if (kt + 1 < t1) deposit(buf ^ 1);
+        lds_barrier();
+    }
+    if (__any(bad)) {
+        // Inf or NaN among the drafted values: added element by element to the
+        // rows whose path holds the slot.
+        for (int64_t slot = max(t0 * TILE, past); slot < min(t1 * TILE, n); ++slot) {
+            const int a = (int) (slot - past);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                if (!(path[tok[i]][a >> 5] >> (a & 31) & 1)) continue;
+                const int row = min(row0 + i * 16 + c16, rows - 1);
+                const float pr = tree_weight(p, b, hk * group + row / p.tq, tok[i], kb + slot * DH, DH, m[i]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t v = vb[(int64_t) (d * 16 + 4 * g + e) * p.vt_ld + slot];
+                        if (not_finite_bf16(v)) o[i][d][e] += pr * bf16_to_f32(v);
+                    }
+            }
         }
     }
-    uint16_t * y = p.out + ((b * p.tq + row % p.tq) * p.heads + hk * group + row / p.tq) * DH + lane * V;
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int v = 0; v < V; ++v) y[v] = m == -INFINITY ? 0 : f32_to_bf16(acc[v] * inv);
+    for (int i = 0; i < NR; ++i) {
+        const int row = row0 + i * 16 + c16;
+        const float sum = sum_xor32(sum_xor16(l[i]));
+        if (row >= rows) continue;
+        const int pr = parents[tok[i]];
+        const bool none = !(pr >= -1 && pr < p.tq) || (sum == 0.0f && m[i] == -INFINITY);
+        if (p.po) {
+            const int64_t at = ((int64_t) u * p.kv_heads + hk) * rows + row;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *(f32x4_t *) (p.po + at * DH + d * 16 + 4 * g) = o[i][d];
+            if (g == 0) {
+                p.pml[2 * at] = none ? -INFINITY : m[i] == -INFINITY ? 0.0f : m[i];
+                p.pml[2 * at + 1] = none ? 0.0f : sum;
+            }
+        } else {
+            const float inv = none ? 0.0f : 1.0f / sum;
+            uint16_t * y = p.out + (((int64_t) b * p.tq + tok[i]) * p.heads + hk * group + row / p.tq) * DH + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                *(uint32_t *) (y + d * 16) = none ? 0u : pack_bf16x2(o[i][d][0] * inv, o[i][d][1] * inv);
+                *(uint32_t *) (y + d * 16 + 2) = none ? 0u : pack_bf16x2(o[i][d][2] * inv, o[i][d][3] * inv);
+            }
+        }
+    }
 }
 
-template <int DH, int NR, int HF>
-static hipError_t run(TreeParams & p, const TreeArgs & a, hipStream_t s) {
-    const int64_t bz = a.batch * a.kv_heads, rows = a.heads / a.kv_heads * a.tq, rt = (rows + 16 * NR - 1) / (16 * NR);
-    if (bz > 65535 || rt > 65535) return hipErrorInvalidValue;
-    // Splits: two workgroups per CU when the cache is long enough for each to
-    // have eight tiles, as far as the workspace holds their results.
-    const int64_t tiles = (a.capacity + 32 * HF - 1) / (32 * HF);
-    int64_t splits = std::min<int64_t>(512 / std::max<int64_t>(bz * rt, 1), tiles / 8);
-    const size_t per = (size_t) (bz * rows) * (DH + 2) * 4;
-    if (!a.ws) splits = 1;
-    else splits = std::min<int64_t>(splits, (int64_t) (a.ws_bytes / std::max<size_t>(per, 1)));
-    if (splits < 2) splits = 1;
-    p.splits = (int32_t) splits;
-    if (splits > 1) {
-        p.po = (float *) a.ws;
-        p.pml = p.po + bz * rows * splits * DH;
+// out = sum_s po_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): a workgroup per row, its
+// threads DH / 4 pieces of four values by 1024 / DH groups of splits, whose
+// sums are added in order.
+template <int DH>
+__global__ __launch_bounds__(256) void tree_attn_join(TreeParams p) {
+    constexpr int PC = DH / 4, GR = 256 / PC;
+    __shared__ __align__(16) f32x4_t acc[GR][PC];
+    __shared__ float part[GR];
+    const int piece = threadIdx.x % PC, gr = threadIdx.x / PC;
+    const int group = p.heads / p.kv_heads, rows = group * p.tq;
+    const uint32_t bz = blockIdx.x / (uint32_t) rows;
+    const int row = (int) (blockIdx.x - bz * (uint32_t) rows);
+    const int64_t b = bz / (uint32_t) p.kv_heads;
+    const int hk = (int) (bz - (uint32_t) b * (uint32_t) p.kv_heads);
+    const TreeUnit unit = tree_unit(p, 0, (int) b);
+    const int64_t step = (int64_t) p.kv_heads * rows, at = unit.first * step + hk * rows + row;
+    float m = -INFINITY;
+    for (int s = threadIdx.x & 63; s < unit.count; s += 64) m = fmaxf(m, p.pml[2 * (at + s * step)]);
+    m = wave_max(m);
+    const float bm = m == -INFINITY ? 0.0f : m;
+    f32x4_t v = {0, 0, 0, 0};
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int s = gr; s < unit.count; s += GR) {
+        const float f = __builtin_amdgcn_exp2f(p.pml[2 * (at + s * step)] - bm);
+        const f32x4_t o = *(const f32x4_t *) (p.po + (at + s * step) * DH + piece * 4);
+        sum += p.pml[2 * (at + s * step) + 1] * f;
+        // A unit without a slot of this row (f = 0) holds zeros.
+        v += o * f;
     }
-    hipLaunchKernelGGL((tree_attn_part<DH, NR, HF>), dim3((unsigned) splits, (unsigned) rt, (unsigned) bz),
-                       dim3(kTreeWaves * 64), 0, s, p);
-    if (splits > 1)
-        hipLaunchKernelGGL(tree_attn_join<DH>, dim3((unsigned) ((bz * rows + 3) / 4)), dim3(256), 0, s, p, bz * rows);
+    acc[gr][piece] = v;
+    if (piece == 0) part[gr] = sum;
+    __syncthreads();
+    if (gr) return;
+    sum = part[0];
+#pragma unroll
+    for (int k = 1; k < GR; ++k) {
+        v += acc[k][piece];
+        sum += part[k];
+    }
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
+    uint16_t * y = p.out + ((b * p.tq + row % p.tq) * p.heads + hk * group + row / p.tq) * DH + piece * 4;
+    const bool none = m == -INFINITY;
+    *(uint32_t *) y = none ? 0u : pack_bf16x2(v[0] * inv, v[1] * inv);
+    *(uint32_t *) (y + 2) = none ? 0u : pack_bf16x2(v[2] * inv, v[3] * inv);
+}
+
+// Units: `wgs` workgroups in all where each has four tiles or more, as far as
+// the workspace holds their results.
+static void plan(TreeParams & p, const TreeArgs & a, int64_t row_tiles, int64_t wgs) {
+    const int64_t rows = a.heads / a.kv_heads * a.tq, tiles = (a.capacity + kTreeTile - 1) / kTreeTile;
+    int64_t units = std::min<int64_t>(wgs / (a.kv_heads * row_tiles), a.batch * std::max<int64_t>(tiles / 4, 1));
+    const size_t per = (size_t) (a.kv_heads * rows) * (size_t) (a.head_dim + 2) * 4;
+    if (!a.ws || a.ws_bytes / per < (size_t) units) units = a.ws ? (int64_t) (a.ws_bytes / per) : 0;
+    p.even = a.batch > 64 || (uint64_t) units * (uint64_t) tiles * (uint64_t) a.batch > 0xffffffffull;
+    if (p.even) units = units / a.batch * a.batch;
+    p.units = (int32_t) std::max<int64_t>(units, a.batch);
+    if (p.units > a.batch) {
+        p.po = (float *) a.ws;
+        p.pml = p.po + (int64_t) p.units * a.kv_heads * rows * a.head_dim;
+    }
+}
+
+template <int DH>
+static hipError_t launch(void (*kernel)(TreeParams), int R, int threads, int64_t target, TreeParams & p,
+                         const TreeArgs & a, hipStream_t s) {
+    const int64_t rows = a.heads / a.kv_heads * a.tq, rt = (rows + R - 1) / R;
+    plan(p, a, rt, target);
+    const int64_t wgs = ((int64_t) p.units * a.kv_heads + 7) / 8 * 8 * rt, joins = a.batch * a.kv_heads * rows;
+    if (wgs > 0x7fffffff || joins > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kernel, dim3((unsigned) wgs), dim3((unsigned) threads), 0, s, p);
+    if (p.po) hipLaunchKernelGGL(tree_attn_join<DH>, dim3((unsigned) joins), dim3(256), 0, s, p);
     return hipGetLastError();
+}
+
+template <int DH, int NR>
+static hipError_t run_rows(TreeParams & p, const TreeArgs & a, hipStream_t s) {
+    return launch<DH>(tree_attn_rows<DH, NR>, NR * 16, kTreeWaves * 64, 768, p, a, s);
+}
+template <int DH, int NR, int W>
+static hipError_t run_many(TreeParams & p, const TreeArgs & a, hipStream_t s) {
+    return launch<DH>(tree_attn_many<DH, NR, W>, W * NR * 16, W * 64, 256, p, a, s);
 }
 
 hipError_t launch_tree_attn(const TreeArgs & a, hipStream_t s) {
     if (a.tq <= 0 || a.batch <= 0) return hipSuccess;
-    if (a.tq > kTreeMax || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.vt_ld % 8 != 0 ||
-        a.vt_ld < a.capacity || a.capacity <= 0)
+    if (a.tq > kTreeMax || a.batch > 0x7fffffff / std::max<int64_t>(a.kv_heads, 1) || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.vt_ld % 8 != 0 ||
+        a.vt_ld < a.capacity || a.capacity <= 0 || a.capacity > 0x7fffffff)
         return hipErrorInvalidValue;
     TreeParams p{};
     p.q = (const uint16_t *) a.q;
@@ -378,14 +720,28 @@ hipError_t launch_tree_attn(const TreeArgs & a, hipStream_t s) {
     p.heads = (int32_t) a.heads;
     p.kv_heads = (int32_t) a.kv_heads;
     p.tq = (int32_t) a.tq;
-    p.scale = a.scale * 1.4426950408889634f;
+    p.batch = (int32_t) a.batch;
+    // The kernels take a positive scale: a negative one turns Q's signs, zero
+    // makes Q zero.
+    p.scale = a.scale == 0.0f ? 1.0f : std::fabs(a.scale) * 1.4426950408889634f;
+    p.q_and = a.scale == 0.0f ? 0u : 0xffffffffu;
+    p.q_xor = a.scale < 0.0f ? 0x80008000u : 0u;
     const int64_t rows = a.heads / a.kv_heads * a.tq;
     switch (a.head_dim) {
         case 64:
-            return rows <= 16 ? run<64, 1, 2>(p, a, s) : rows <= 32 ? run<64, 2, 2>(p, a, s) : run<64, 4, 2>(p, a, s);
+            if (rows <= 16) return run_rows<64, 1>(p, a, s);
+            if (rows <= 32) return run_rows<64, 2>(p, a, s);
+            if (rows <= 48) return run_rows<64, 3>(p, a, s);
+            return rows <= 64 ? run_rows<64, 4>(p, a, s) : run_many<64, 2, 8>(p, a, s);
         case 128:
-            return rows <= 16 ? run<128, 1, 2>(p, a, s) : rows <= 32 ? run<128, 2, 2>(p, a, s) : run<128, 4, 1>(p, a, s);
-        case 256: return rows <= 16 ? run<256, 1, 1>(p, a, s) : run<256, 2, 1>(p, a, s);
+            if (rows <= 16) return run_rows<128, 1>(p, a, s);
+            if (rows <= 32) return run_rows<128, 2>(p, a, s);
+            if (rows <= 48) return run_rows<128, 3>(p, a, s);
+            return rows <= 64 ? run_rows<128, 4>(p, a, s) : run_many<128, 2, 8>(p, a, s);
+        case 256:
+            if (rows <= 16) return run_rows<256, 1>(p, a, s);
+            if (rows <= 32) return run_rows<256, 2>(p, a, s);
+            return rows <= 48 ? run_rows<256, 3>(p, a, s) : run_many<256, 1, 8>(p, a, s);
         default: return hipErrorInvalidValue;
     }
 }
