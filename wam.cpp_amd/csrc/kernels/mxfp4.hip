@@ -27,6 +27,15 @@ struct __attribute__((packed, aligned(1))) any8 {
     uint32_t v[2];
 };
 
+// A barrier that waits for this wave's LDS accesses alone: loads into registers
+// stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Eight consecutive values as f32.
@@ -394,6 +403,188 @@ static void launch_few(const MxParams & p, bool xf32, hipStream_t s) {
     else hipLaunchKernelGGL((mx_few<RG, NT, false>), grid, dim3(kMxWaves * 64), 0, s, p);
 }
 
+// Many tokens: matrix-core bound.  Eight waves, 2 along the weight rows by 4
+// along the tokens, each RG x NT tiles of 16 x 16 (so RG * 32 rows by NT * 64
+// tokens a workgroup).  The weight stays in its 4 bits down to the register
+// that becomes the operand: a step of 128 values is 4 blocks a row, whose codes
+// lie in LDS as [row][pair of blocks][g][block of the pair], so that one
+// 8-byte read gives lane (r, g) dword g of both blocks of a pair.  Such a dword
+// expands to values (4g + t, 16 + 4g + t), t = 0..3, of its block, and x is
+// written to LDS in that order (two 16-byte pieces 16 values apart, interleaved
+// on the way), half a step at a time.  Both go through registers into one of
+// two buffers while the other is multiplied: one barrier per half step.
+template <bool XF32>
+struct MxPiece {  // eight consecutive activations
+    any16 v[XF32 ? 2 : 1];
+};
+
+template <int RG, int NT, bool XF32>
+__global__ __launch_bounds__(512) void mx_tile(MxParams p) {
+    constexpr int BM = RG * 32, BN = NT * 64, XP = BN * 8 / 512;  // x pieces of a thread per half step
+    constexpr int WB = (BM * 4 + 511) / 512;                      // weight blocks of a thread per step
+    static_assert(XP % 2 == 0, "pieces come in pairs");
+    __shared__ __align__(16) uint32_t wl[2][BM * 16];
+    __shared__ __align__(16) float sl[2][BM * 4];
+    __shared__ __align__(16) uint32_t xl[2][BN * 32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4, wm = wave >> 2, wn = wave & 3;
+    const int64_t m0 = (int64_t) blockIdx.x * BM, n0 = (int64_t) blockIdx.y * BN;
+    const int s0 = (int) blockIdx.z * p.steps, s1 = min(s0 + p.steps, (p.kb + 3) / 4);
+    constexpr int xs = XF32 ? 4 : 2;
+
+    // Weight blocks: thread t takes block t % 4 of rows t / 4, t / 4 + 128, ...
+    const int wkb = threadIdx.x & 3, wrow = threadIdx.x >> 2;
+    const uint8_t * wsrc[WB];
+#pragma unroll
+    for (int j = 0; j < WB; ++j) wsrc[j] = p.w + min(m0 + wrow + j * 128, p.M - 1) * p.ws;
+    any16 wr[WB];
+    uint32_t wsc[WB];
+    auto request_w = [&](int s) {
+        const int kb = 4 * s + wkb;
+        const int64_t at = min(kb, p.kb - 1) * (int64_t) kMxBytes;
+#pragma unroll
+        for (int j = 0; j < WB; ++j) {
+            wr[j] = *(const any16 *) (wsrc[j] + at + 1);
+            wsc[j] = wsrc[j][at];
+            if (kb >= p.kb) {
+                wsc[j] = 0;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) wr[j].v[d] = 0;
+            }
+        }
+    };
+    auto deposit_w = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < WB; ++j) {
+            const int row = wrow + j * 128;
+            if (BM % 128 != 0 && row >= BM) break;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) wl[buf][row * 16 + (wkb >> 1) * 8 + d * 2 + (wkb & 1)] = wr[j].v[d];
+            sl[buf][row * 4 + wkb] = mx_scale(wsc[j]);
+        }
+    };
+    // Activations: pair q of a thread is the pieces at 8c and 16 + 8c of a
+    // 32-value block, c = 0, 1.
+    MxPiece<XF32> xr[XP];
+    const char * xsrc[XP / 2];
+    int xpos[XP / 2];
+#pragma unroll
+    for (int q = 0; q < XP / 2; ++q) {
+        const int e = threadIdx.x + q * 512, row = e >> 2, i = (e >> 1) & 1, c = e & 1;
+        xsrc[q] = (const char *) p.x + (min(n0 + row, p.N - 1) * p.ldx + i * 32 + c * 8) * xs;
+        xpos[q] = row * 8 + ((i * 4 + c * 2) ^ ((row >> 1) & 7));  // 16-byte slot of operand g = 2c; g + 1 in slot ^ 1
+    }
+    auto request_x = [&](int h) {  // half step h: blocks 2h, 2h + 1
+#pragma unroll
+        for (int q = 0; q < XP / 2; ++q) {
+            const int kb = 2 * h + ((threadIdx.x >> 1) & 1);
+            const bool in = kb < p.kb;
+            const char * a = xsrc[q] + (in ? (int64_t) h * 64 : 0) * xs - (in ? 0 : ((threadIdx.x >> 1) & 1) * 32 * xs);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < (XF32 ? 2 : 1); ++v) {
+                    xr[2 * q + u].v[v] = *(const any16 *) (a + u * 16 * xs + v * 16);
+                    if (!in) {
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) xr[2 * q + u].v[v].v[d] = 0;
+                    }
+                }
+        }
+    };
+    auto deposit_x = [&](int buf) {
+#pragma unroll
+        for (int q = 0; q < XP / 2; ++q) {
+            uint32_t lo[4], hi[4];
+            if constexpr (XF32) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const any16 &a = xr[2 * q].v[d >> 1], &b = xr[2 * q + 1].v[d >> 1];
+                    lo[d] = pack_bf16x2(__uint_as_float(a.v[2 * (d & 1)]), __uint_as_float(a.v[2 * (d & 1) + 1]));
+                    hi[d] = pack_bf16x2(__uint_as_float(b.v[2 * (d & 1)]), __uint_as_float(b.v[2 * (d & 1) + 1]));
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    lo[d] = xr[2 * q].v[0].v[d];
+                    hi[d] = xr[2 * q + 1].v[0].v[d];
+                }
+            }
+            bf16x8_t * dst = (bf16x8_t *) xl[buf];
+            dst[xpos[q]] = mx_pair(lo[0], lo[1], hi[0], hi[1]);
+            dst[xpos[q] ^ 1] = mx_pair(lo[2], lo[3], hi[2], hi[3]);
+        }
+    };
+
+    f32x4_t acc[RG][NT];
+#pragma unroll
+    for (int i = 0; i < RG; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
+    auto multiply = [&](int wbuf, int half, int xbuf) {
+        bf16x8_t b[2][NT];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int row = (wn * NT + j) * 16 + c16;
+                b[i][j] = ((const bf16x8_t *) xl[xbuf])[row * 8 + ((i * 4 + g) ^ ((row >> 1) & 7))];
+            }
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+            const int row = (wm * RG + r) * 16 + c16;
+            const uint2 d = *(const uint2 *) &wl[wbuf][row * 16 + half * 8 + g * 2];
+            const float2 sc = *(const float2 *) &sl[wbuf][row * 4 + half * 2];
+            const bf16x8_t a0 = mx_frag(d.x, sc.x), a1 = mx_frag(d.y, sc.y);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b[0][j], acc[r][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b[1][j], acc[r][j], 0, 0, 0);
+        }
+    };
+    if (s0 < s1) {
+        request_w(s0);
+        request_x(2 * s0);
+        deposit_w(0);
+        deposit_x(0);
+    }
+    lds_barrier();
+    for (int s = s0; s < s1; ++s) {
+        const int wb = (s - s0) & 1;
+        request_x(2 * s + 1);
+        if (s + 1 < s1) request_w(s + 1);
+        multiply(wb, 0, 0);
+        deposit_x(1);
+        lds_barrier();
+        if (s + 1 < s1) request_x(2 * s + 2);
+        multiply(wb, 1, 1);
+        if (s + 1 < s1) {
+            deposit_x(0);
+            deposit_w(wb ^ 1);
+        }
+        lds_barrier();
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + (wn * NT + j) * 16 + c16;
+        if (n >= p.N) continue;
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+            const int64_t m = m0 + (wm * RG + r) * 16 + 4 * g;
+            if (m >= p.M) continue;
+            const float o[4] = {acc[r][j][0], acc[r][j][1], acc[r][j][2], acc[r][j][3]};
+            mx_store4(p, n, m, o);
+        }
+    }
+}
+
+template <int RG, int NT>
+static void launch_tile(const MxParams & p, bool xf32, hipStream_t s) {
+    const dim3 grid((unsigned) ((p.M + RG * 32 - 1) / (RG * 32)), (unsigned) ((p.N + NT * 64 - 1) / (NT * 64)), 1);
+    if (xf32) hipLaunchKernelGGL((mx_tile<RG, NT, true>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((mx_tile<RG, NT, false>), grid, dim3(512), 0, s, p);
+}
+
 hipError_t launch_mx_quantize(const void * x, int32_t x_type, int64_t ldx, void * q, int64_t rows, int64_t cols,
                               hipStream_t s) {
     const int64_t rb = cols / 32, blocks = rows * rb;
@@ -451,7 +642,9 @@ hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     const bool xf32 = a.x_type == WAMX_TYPE_F32;
     if (a.N <= 16) launch_few<1, 1>(p, xf32, s);
     else if (a.N <= 32) launch_few<1, 2>(p, xf32, s);
-    else launch_few<2, 4>(p, xf32, s);
+    else if (a.N <= 64) launch_few<2, 4>(p, xf32, s);
+    else if (a.N <= 600) launch_tile<4, 2>(p, xf32, s);
+    else launch_tile<8, 4>(p, xf32, s);
     return hipGetLastError();
 }
 
