@@ -36,6 +36,30 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// A block read as the five aligned dwords that hold its 17 bytes, `mis` bytes
+// into the first (every dword holds a byte of the block, so none lies outside
+// the tensor's pages).  As 16 + 1 bytes at their odd addresses the few-token
+// products took 7.1 and 32 us where these take 5.3 and 27 (4096 x 1 x 4096,
+// 14336 x 48 x 4096).  Blocks four apart have one `mis`.
+struct __attribute__((packed, aligned(4))) dwords4 {
+    uint32_t v[4];
+};
+struct MxBlock {
+    dwords4 lo;
+    uint32_t hi;
+};
+__device__ __forceinline__ MxBlock mx_load(const void * aligned) {
+    return {*(const dwords4 *) aligned, ((const uint32_t *) aligned)[4]};
+}
+__device__ __forceinline__ uint32_t mx_select(uint32_t mis) { return 0x04030201u + mis * 0x01010101u; }
+__device__ __forceinline__ uint32_t mx_exponent(const MxBlock & b, uint32_t mis) {
+    return (b.lo.v[0] >> (8 * mis)) & 255u;
+}
+// Dword i of the codes.
+__device__ __forceinline__ uint32_t mx_codes(const MxBlock & b, int i, uint32_t select) {
+    return __builtin_amdgcn_perm(i < 3 ? b.lo.v[i + 1] : b.hi, b.lo.v[i], select);
+}
+
 __device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Eight consecutive values as f32.
@@ -212,8 +236,8 @@ struct MxParams {
     int64_t M, N;
     int kb;  // blocks of a row
     int32_t y_f32, epi;
-    float * part;  // K-split planes [split][N][M], or null
-    int steps;     // K steps of 128 of one split
+    int64_t plane;  // bytes from one K split's f32 plane to the next's (y is the first), or 0
+    int steps;      // K steps of 128 of one split
 };
 
 // Four outputs y[n][m .. m + 3] with the rounding points of the LINEAR
@@ -293,92 +317,127 @@ constexpr int kMxWaves = 8;
 
 template <int RG, int NT, bool XF32>
 __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
-    __shared__ __align__(16) f32x4_t red[kMxWaves][RG * NT][64];
+    // A wave's x of one step, [token][16-byte piece]; after the last step the
+    // waves' sums.
+    constexpr int XB = NT * 16 * 256, RB = RG * NT * 64 * 16;
+    __shared__ __align__(16) uint8_t lds[kMxWaves * (XB > RB ? XB : RB)];
+    f32x4_t (*red)[RG * NT][64] = (f32x4_t (*)[RG * NT][64]) lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int64_t m0 = (int64_t) blockIdx.x * (16 * RG), n0 = (int64_t) blockIdx.y * (16 * NT);
     const int s0 = (int) blockIdx.z * p.steps, s1 = min(s0 + p.steps, (p.kb + 3) / 4);
+    p.y = (char *) p.y + blockIdx.z * p.plane;
 
-    const uint8_t * w[RG];
-    const char * x[NT];
+    const char * w[RG];
+    uint32_t mis[RG];
+    const char * x[NT * 4];
     constexpr int xs = XF32 ? 4 : 2;
 #pragma unroll
-    for (int i = 0; i < RG; ++i) w[i] = p.w + min(m0 + i * 16 + r, p.M - 1) * p.ws;
+    for (int i = 0; i < RG; ++i) {
+        // Rows of fewer than four blocks: their last one for the lanes past it.
+        w[i] = (const char *) p.w + min(m0 + i * 16 + r, p.M - 1) * p.ws + min(g, p.kb - 1) * (int) kMxBytes;
+        mis[i] = (uint32_t) (uintptr_t) w[i] & 3;
+        w[i] -= mis[i];
+    }
+    // Sixteen lanes read the 256 bytes of a token's step (twice that in f32), a
+    // lane four tokens.
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = (const char *) p.x + min(n0 + j * 16 + r, p.N - 1) * p.ldx * xs;
+    for (int j = 0; j < NT * 4; ++j)
+        x[j] = (const char *) p.x + (min(n0 + j * 4 + g, p.N - 1) * p.ldx + r * 8) * xs;
+    uint4 * mine = (uint4 *) (lds + wave * XB);
 
-    struct Step {
-        any16 w[RG];
-        uint32_t e[RG];
-        uint32_t x[NT][16];
+    // The next step is requested when this one's x lies in LDS.
+    MxBlock wr[2][RG];
+    any16 xr[NT * 4][XF32 ? 2 : 1];
+    auto load = [&](int s, MxBlock * t) {
+        // A lane past the row's last block repeats its block of the step before.
+        const int64_t o = (int64_t) (s - (s > 0 && 4 * s + g >= p.kb)) * (4 * kMxBytes);
+#pragma unroll
+        for (int i = 0; i < RG; ++i) t[i] = mx_load(w[i] + o);
+        const int64_t xo = (4 * s + (r >> 2) < p.kb ? (int64_t) s * 128 : -r * 8) * xs;  // past the row: its start
+#pragma unroll
+        for (int j = 0; j < NT * 4; ++j)
+#pragma unroll
+            for (int v = 0; v < (XF32 ? 2 : 1); ++v) xr[j][v] = *(const any16 *) (x[j] + xo + 16 * v);
     };
-    auto load = [&](int s, Step & t) {
-        const int kb = 4 * s + g;
-        const bool in = kb < p.kb;
-        const int64_t at = in ? kb : p.kb - 1;
-#pragma unroll
-        for (int i = 0; i < RG; ++i) {
-            const uint8_t * b = w[i] + at * kMxBytes;
-            t.w[i] = *(const any16 *) (b + 1);
-            t.e[i] = b[0];
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            if constexpr (XF32) {
-                const char * b = x[j] + at * 128;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const any16 a = *(const any16 *) (b + 16 * c);
-                    t.x[j][2 * c] = pack_bf16x2(__uint_as_float(a.v[0]), __uint_as_float(a.v[1]));
-                    t.x[j][2 * c + 1] = pack_bf16x2(__uint_as_float(a.v[2]), __uint_as_float(a.v[3]));
-                }
-            } else {
-                const char * b = x[j] + at * 64;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const any16 a = *(const any16 *) (b + 16 * c);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) t.x[j][4 * c + d] = a.v[d];
-                }
-            }
-        }
-        if (!in) {
-            // Past the row's last block: nothing times nothing.
-#pragma unroll
-            for (int i = 0; i < RG; ++i) {
-                t.e[i] = 0;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) t.w[i].v[d] = 0;
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int d = 0; d < 16; ++d) t.x[j][d] = 0;
-        }
-    };
-
     f32x4_t acc[RG][NT];
 #pragma unroll
     for (int i = 0; i < RG; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
-    Step cur;
-    for (int s = s0 + wave; s < s1; s += kMxWaves) {
-        load(s, cur);
+    auto multiply = [&](int s, int next, MxBlock * t, MxBlock * tn) {
+        // Through LDS into operand order: piece q of token n in slot q ^ (n % 16),
+        // so that the 16 tokens of a read lie in different banks.
+        const bool tail = 4 * s + 4 > p.kb;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            bf16x8_t b[NT];
+        for (int j = 0; j < NT * 4; ++j) {
+            uint4 v;
+            if constexpr (XF32) {
+                const any16 &a = xr[j][0], &b = xr[j][1];
+                v = make_uint4(pack_bf16x2(__uint_as_float(a.v[0]), __uint_as_float(a.v[1])),
+                               pack_bf16x2(__uint_as_float(a.v[2]), __uint_as_float(a.v[3])),
+                               pack_bf16x2(__uint_as_float(b.v[0]), __uint_as_float(b.v[1])),
+                               pack_bf16x2(__uint_as_float(b.v[2]), __uint_as_float(b.v[3])));
+            } else {
+                v = make_uint4(xr[j][0].v[0], xr[j][0].v[1], xr[j][0].v[2], xr[j][0].v[3]);
+            }
+            const int n = j * 4 + g;
+            mine[n * 16 + (r ^ (n & 15))] = v;
+        }
+        if (tail && 4 * s + (r >> 2) >= p.kb) {  // past the row's last block: nothing times nothing
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                b[j] = mx_pair(cur.x[j][2 * d], cur.x[j][2 * d + 1], cur.x[j][8 + 2 * d], cur.x[j][8 + 2 * d + 1]);
+            for (int j = 0; j < NT * 4; ++j) mine[(j * 4 + g) * 16 + (r ^ ((j * 4 + g) & 15))] = make_uint4(0, 0, 0, 0);
+        }
+        if (tail && 4 * s + g >= p.kb) {
 #pragma unroll
             for (int i = 0; i < RG; ++i) {
-                const bf16x8_t a = mx_frag(cur.w[i].v[d], mx_scale(cur.e[i]));
+                t[i].hi = 0;
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[j], acc[i][j], 0, 0, 0);
+                for (int d = 0; d < 4; ++d) t[i].lo.v[d] = 0;
             }
         }
+        if (next >= 0) load(next, tn);
+        __builtin_amdgcn_wave_barrier();
+        // Dwords 2h and 2h + 1 of the codes meet pieces h and h + 2 of block g.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint4 lo[NT], hi[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                lo[j] = mine[(j * 16 + r) * 16 + ((4 * g + h) ^ r)];
+                hi[j] = mine[(j * 16 + r) * 16 + ((4 * g + h + 2) ^ r)];
+            }
+#pragma unroll
+            for (int d = 2 * h; d < 2 * h + 2; ++d) {
+                bf16x8_t b[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    b[j] = d & 1 ? mx_pair(lo[j].z, lo[j].w, hi[j].z, hi[j].w) : mx_pair(lo[j].x, lo[j].y, hi[j].x, hi[j].y);
+#pragma unroll
+                for (int i = 0; i < RG; ++i) {
+                    const bf16x8_t a = mx_frag(mx_codes(t[i], d, mx_select(mis[i])), mx_scale(mx_exponent(t[i], mis[i])));
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[j], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    // Workgroups begin at different steps: rows of x lie a power of two apart as
+    // often as not, where one step of all rows is one channel of the L2.
+    const int ns = s1 - s0, turn = (int) (blockIdx.x % (uint32_t) ns);
+    auto at = [&](int k) { return s0 + (k + turn < ns ? k + turn : k + turn - ns); };
+    int k = wave;
+    if (k < ns) load(at(k), wr[0]);
+    while (k < ns) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (k >= ns) break;
+            multiply(at(k), k + kMxWaves < ns ? at(k + kMxWaves) : -1, wr[q], wr[q ^ 1]);
+            k += kMxWaves;
+        }
     }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < RG; ++i)
 #pragma unroll
@@ -396,123 +455,105 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
     }
 }
 
-template <int RG, int NT>
-static void launch_few(const MxParams & p, bool xf32, hipStream_t s) {
-    const dim3 grid((unsigned) ((p.M + 16 * RG - 1) / (16 * RG)), (unsigned) ((p.N + 16 * NT - 1) / (16 * NT)), 1);
-    if (xf32) hipLaunchKernelGGL((mx_few<RG, NT, true>), grid, dim3(kMxWaves * 64), 0, s, p);
-    else hipLaunchKernelGGL((mx_few<RG, NT, false>), grid, dim3(kMxWaves * 64), 0, s, p);
-}
-
 // Many tokens: matrix-core bound.  Eight waves, 2 along the weight rows by 4
 // along the tokens, each RG x NT tiles of 16 x 16 (so RG * 32 rows by NT * 64
 // tokens a workgroup).  The weight stays in its 4 bits down to the register
 // that becomes the operand: a step of 128 values is 4 blocks a row, whose codes
-// lie in LDS as [row][pair of blocks][g][block of the pair], so that one
-// 8-byte read gives lane (r, g) dword g of both blocks of a pair.  Such a dword
+// lie in LDS as [block][row][g], so that a wave's read of dword g of its rows is
+// 256 bytes in a row.  Such a dword
 // expands to values (4g + t, 16 + 4g + t), t = 0..3, of its block, and x is
 // written to LDS in that order (two 16-byte pieces 16 values apart, interleaved
-// on the way), half a step at a time.  Both go through registers into one of
-// two buffers while the other is multiplied: one barrier per half step.
-template <bool XF32>
-struct MxPiece {  // eight consecutive activations
-    any16 v[XF32 ? 2 : 1];
-};
-
-template <int RG, int NT, bool XF32>
-__global__ __launch_bounds__(512) void mx_tile(MxParams p) {
-    constexpr int BM = RG * 32, BN = NT * 64, XP = BN * 8 / 512;  // x pieces of a thread per half step
-    constexpr int WB = (BM * 4 + 511) / 512;                      // weight blocks of a thread per step
-    static_assert(XP % 2 == 0, "pieces come in pairs");
-    __shared__ __align__(16) uint32_t wl[2][BM * 16];
-    __shared__ __align__(16) float sl[2][BM * 4];
+// on the way), half a step at a time.  Both go through registers, requested a
+// step before their use, into one of two LDS buffers while the other is
+// multiplied: one barrier per half step, the writes behind the first row tile's
+// products.
+template <int RG, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
+    constexpr int TH = 64 * WM * WN, BM = RG * 16 * WM, BN = NT * 16 * WN;
+    constexpr int XP = BN * 4 / TH;             // pairs of x pieces of a thread per half step
+    constexpr int WB = (BM * 4 + TH - 1) / TH;  // weight blocks of a thread per step
+    // The four blocks of a row, written by four neighbouring lanes, lie a
+    // quarter of the banks apart.
+    constexpr int WS = (BM + 15) / 16 * 16 + 4, SS = (BM + 63) / 64 * 64 + 16;
+    __shared__ __align__(16) uint32_t wl[2][WS * 16];
+    __shared__ __align__(16) float sl[2][SS * 4];
     __shared__ __align__(16) uint32_t xl[2][BN * 32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c16 = lane & 15, g = lane >> 4, wm = wave >> 2, wn = wave & 3;
+    const int c16 = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
     const int64_t m0 = (int64_t) blockIdx.x * BM, n0 = (int64_t) blockIdx.y * BN;
     const int s0 = (int) blockIdx.z * p.steps, s1 = min(s0 + p.steps, (p.kb + 3) / 4);
-    constexpr int xs = XF32 ? 4 : 2;
+    p.y = (char *) p.y + blockIdx.z * p.plane;
+    // Sources: one address for the workgroup, 32-bit offsets for the lanes (a
+    // tile's rows lie within 4 GB, see launch_mx_product).
+    const char * wbase = (const char *) p.w + m0 * p.ws;
+    const char * xbase = (const char *) p.x + n0 * p.ldx * 2;
 
-    // Weight blocks: thread t takes block t % 4 of rows t / 4, t / 4 + 128, ...
+    // Weight blocks: thread t takes block t % 4 of rows t / 4, t / 4 + TH / 4, ...
     const int wkb = threadIdx.x & 3, wrow = threadIdx.x >> 2;
-    const uint8_t * wsrc[WB];
+    uint32_t woff[WB];
 #pragma unroll
-    for (int j = 0; j < WB; ++j) wsrc[j] = p.w + min(m0 + wrow + j * 128, p.M - 1) * p.ws;
+    for (int j = 0; j < WB; ++j)
+        woff[j] = (uint32_t) min((int64_t) (wrow + j * (TH / 4)), p.M - 1 - m0) * (uint32_t) p.ws;
+    // (Loads at odd addresses: the five dwords of mx_load cost registers that
+    // the large tiles do not have, 14336 x 2048 x 4096 in 224 us against 210.)
     any16 wr[WB];
     uint32_t wsc[WB];
-    auto request_w = [&](int s) {
-        const int kb = 4 * s + wkb;
-        const int64_t at = min(kb, p.kb - 1) * (int64_t) kMxBytes;
+    auto request_w = [&](int s, any16 * r, uint32_t * e) {
+        const uint32_t at = (uint32_t) min(4 * s + wkb, p.kb - 1) * (uint32_t) kMxBytes;
 #pragma unroll
         for (int j = 0; j < WB; ++j) {
-            wr[j] = *(const any16 *) (wsrc[j] + at + 1);
-            wsc[j] = wsrc[j][at];
-            if (kb >= p.kb) {
-                wsc[j] = 0;
+            r[j] = *(const any16 *) (wbase + (woff[j] + at + 1u));
+            e[j] = *(const uint8_t *) (wbase + (woff[j] + at));
+        }
+    };
+    auto deposit_w = [&](int s, int buf, const any16 * r, const uint32_t * e) {
 #pragma unroll
-                for (int d = 0; d < 4; ++d) wr[j].v[d] = 0;
+        for (int j = 0; j < WB; ++j) {
+            const int row = wrow + j * (TH / 4);
+            if (BM % (TH / 4) != 0 && row >= BM) break;
+            ((uint4 *) wl[buf])[wkb * WS + row] = make_uint4(r[j].v[0], r[j].v[1], r[j].v[2], r[j].v[3]);
+            sl[buf][wkb * SS + row] = mx_scale(e[j]);
+        }
+        if (4 * s + 4 > p.kb && 4 * s + wkb >= p.kb) {  // past a row's last block: zeros
+#pragma unroll
+            for (int j = 0; j < WB; ++j) {
+                const int row = wrow + j * (TH / 4);
+                if (BM % (TH / 4) != 0 && row >= BM) break;
+                ((uint4 *) wl[buf])[wkb * WS + row] = make_uint4(0, 0, 0, 0);
+                sl[buf][wkb * SS + row] = 1.0f;
             }
         }
     };
-    auto deposit_w = [&](int buf) {
+    // Activations: a pair is the pieces at 8c and 16 + 8c (c = 0, 1) of block
+    // xi = 0, 1 of a half step.
+    const int xi = (threadIdx.x >> 1) & 1, xc = threadIdx.x & 1;
+    any16 xr[2][XP][2];
+    uint32_t xoff[XP];
+    int xpos[XP];
 #pragma unroll
-        for (int j = 0; j < WB; ++j) {
-            const int row = wrow + j * 128;
-            if (BM % 128 != 0 && row >= BM) break;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) wl[buf][row * 16 + (wkb >> 1) * 8 + d * 2 + (wkb & 1)] = wr[j].v[d];
-            sl[buf][row * 4 + wkb] = mx_scale(wsc[j]);
-        }
-    };
-    // Activations: pair q of a thread is the pieces at 8c and 16 + 8c of a
-    // 32-value block, c = 0, 1.
-    MxPiece<XF32> xr[XP];
-    const char * xsrc[XP / 2];
-    int xpos[XP / 2];
-#pragma unroll
-    for (int q = 0; q < XP / 2; ++q) {
-        const int e = threadIdx.x + q * 512, row = e >> 2, i = (e >> 1) & 1, c = e & 1;
-        xsrc[q] = (const char *) p.x + (min(n0 + row, p.N - 1) * p.ldx + i * 32 + c * 8) * xs;
-        xpos[q] = row * 8 + ((i * 4 + c * 2) ^ ((row >> 1) & 7));  // 16-byte slot of operand g = 2c; g + 1 in slot ^ 1
+    for (int q = 0; q < XP; ++q) {
+        const int row = (threadIdx.x >> 2) + q * (TH / 4);
+        xoff[q] = ((uint32_t) min((int64_t) row, p.N - 1 - n0) * (uint32_t) p.ldx + (uint32_t) xc * 8) * 2;
+        xpos[q] = row * 8 + ((xi * 4 + xc * 2) ^ ((row >> 1) & 7));  // slot of operand g = 2c; g + 1 in slot ^ 1
     }
-    auto request_x = [&](int h) {  // half step h: blocks 2h, 2h + 1
+    auto request_x = [&](int h, any16 (*r)[2]) {  // half step h: blocks 2h, 2h + 1
+        const uint32_t at = (uint32_t) min(2 * h + xi, p.kb - 1) * 64u;
 #pragma unroll
-        for (int q = 0; q < XP / 2; ++q) {
-            const int kb = 2 * h + ((threadIdx.x >> 1) & 1);
-            const bool in = kb < p.kb;
-            const char * a = xsrc[q] + (in ? (int64_t) h * 64 : 0) * xs - (in ? 0 : ((threadIdx.x >> 1) & 1) * 32 * xs);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int v = 0; v < (XF32 ? 2 : 1); ++v) {
-                    xr[2 * q + u].v[v] = *(const any16 *) (a + u * 16 * xs + v * 16);
-                    if (!in) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) xr[2 * q + u].v[v].v[d] = 0;
-                    }
-                }
+        for (int q = 0; q < XP; ++q) {
+            r[q][0] = *(const any16 *) (xbase + (xoff[q] + at));
+            r[q][1] = *(const any16 *) (xbase + (xoff[q] + at + 32u));
         }
     };
-    auto deposit_x = [&](int buf) {
+    auto deposit_x = [&](int h, int buf, any16 (*r)[2]) {
+        bf16x8_t * dst = (bf16x8_t *) xl[buf];
 #pragma unroll
-        for (int q = 0; q < XP / 2; ++q) {
-            uint32_t lo[4], hi[4];
-            if constexpr (XF32) {
+        for (int q = 0; q < XP; ++q) {
+            dst[xpos[q]] = mx_pair(r[q][0].v[0], r[q][0].v[1], r[q][1].v[0], r[q][1].v[1]);
+            dst[xpos[q] ^ 1] = mx_pair(r[q][0].v[2], r[q][0].v[3], r[q][1].v[2], r[q][1].v[3]);
+        }
+        if (2 * h + 2 > p.kb && 2 * h + xi >= p.kb) {
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const any16 &a = xr[2 * q].v[d >> 1], &b = xr[2 * q + 1].v[d >> 1];
-                    lo[d] = pack_bf16x2(__uint_as_float(a.v[2 * (d & 1)]), __uint_as_float(a.v[2 * (d & 1) + 1]));
-                    hi[d] = pack_bf16x2(__uint_as_float(b.v[2 * (d & 1)]), __uint_as_float(b.v[2 * (d & 1) + 1]));
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    lo[d] = xr[2 * q].v[0].v[d];
-                    hi[d] = xr[2 * q + 1].v[0].v[d];
-                }
-            }
-            bf16x8_t * dst = (bf16x8_t *) xl[buf];
-            dst[xpos[q]] = mx_pair(lo[0], lo[1], hi[0], hi[1]);
-            dst[xpos[q] ^ 1] = mx_pair(lo[2], lo[3], hi[2], hi[3]);
+            for (int q = 0; q < XP; ++q) dst[xpos[q]] = dst[xpos[q] ^ 1] = (bf16x8_t){};
         }
     };
 
@@ -521,47 +562,52 @@ __global__ __launch_bounds__(512) void mx_tile(MxParams p) {
     for (int i = 0; i < RG; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
-    auto multiply = [&](int wbuf, int half, int xbuf) {
+    auto multiply = [&](int wbuf, int half, auto && middle) {
         bf16x8_t b[2][NT];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int row = (wn * NT + j) * 16 + c16;
-                b[i][j] = ((const bf16x8_t *) xl[xbuf])[row * 8 + ((i * 4 + g) ^ ((row >> 1) & 7))];
+                b[i][j] = ((const bf16x8_t *) xl[half])[row * 8 + ((i * 4 + g) ^ ((row >> 1) & 7))];
             }
 #pragma unroll
         for (int r = 0; r < RG; ++r) {
-            const int row = (wm * RG + r) * 16 + c16;
-            const uint2 d = *(const uint2 *) &wl[wbuf][row * 16 + half * 8 + g * 2];
-            const float2 sc = *(const float2 *) &sl[wbuf][row * 4 + half * 2];
-            const bf16x8_t a0 = mx_frag(d.x, sc.x), a1 = mx_frag(d.y, sc.y);
+            if (r == 1) middle();
+            const int row = (wm * RG + r) * 16 + c16, k = half * 2;
+            const bf16x8_t a0 = mx_frag(wl[wbuf][(k * WS + row) * 4 + g], sl[wbuf][k * SS + row]);
+            const bf16x8_t a1 = mx_frag(wl[wbuf][((k + 1) * WS + row) * 4 + g], sl[wbuf][(k + 1) * SS + row]);
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, b[0][j], acc[r][j], 0, 0, 0);
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, b[1][j], acc[r][j], 0, 0, 0);
         }
     };
+    // Requests past the last step repeat its addresses (requested, not used).
+    const int last = s1 - 1;
     if (s0 < s1) {
-        request_w(s0);
-        request_x(2 * s0);
-        deposit_w(0);
-        deposit_x(0);
+        request_w(s0, wr, wsc);
+        request_x(2 * s0, xr[0]);
+        request_x(2 * s0 + 1, xr[1]);
+        deposit_w(s0, 0, wr, wsc);
+        deposit_x(2 * s0, 0, xr[0]);
+        request_w(min(s0 + 1, last), wr, wsc);
+        request_x(2 * min(s0 + 1, last), xr[0]);
     }
     lds_barrier();
     for (int s = s0; s < s1; ++s) {
         const int wb = (s - s0) & 1;
-        request_x(2 * s + 1);
-        if (s + 1 < s1) request_w(s + 1);
-        multiply(wb, 0, 0);
-        deposit_x(1);
+        multiply(wb, 0, [&]() {
+            deposit_x(2 * s + 1, 1, xr[1]);
+            request_x(2 * min(s + 1, last) + 1, xr[1]);
+        });
         lds_barrier();
-        if (s + 1 < s1) request_x(2 * s + 2);
-        multiply(wb, 1, 1);
-        if (s + 1 < s1) {
-            deposit_x(0);
-            deposit_w(wb ^ 1);
-        }
+        multiply(wb, 1, [&]() {
+            deposit_x(2 * s + 2, 0, xr[0]);
+            deposit_w(s + 1, wb ^ 1, wr, wsc);
+            request_x(2 * min(s + 2, last), xr[0]);
+            request_w(min(s + 2, last), wr, wsc);
+        });
         lds_barrier();
     }
 #pragma unroll
@@ -578,11 +624,139 @@ __global__ __launch_bounds__(512) void mx_tile(MxParams p) {
     }
 }
 
+// f32 rows rounded to bf16, one after another.
+__global__ __launch_bounds__(256) void mx_round_rows(const float * __restrict__ x, int64_t ldx, uint16_t * __restrict__ y,
+                                                     int64_t rows, int row_pieces) {
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * row_pieces) return;
+    const int64_t r = i / row_pieces;
+    float v[8];
+    load8(x + r * ldx + (i - r * row_pieces) * 8, v);
+    store8(y + i * 8, v);
+}
+
+// The K splits' planes, added in order, with the product's epilogue.
+__global__ __launch_bounds__(256) void mx_reduce(MxParams p, const float * __restrict__ part, int splits) {
+    const int64_t quads = (p.M + 3) / 4, i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.N * quads) return;
+    const int64_t n = i / quads, m = (i - n * quads) * 4;
+    float v[4] = {0, 0, 0, 0};
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (m + r < p.M) v[r] += part[(s * p.N + n) * p.M + m + r];
+    mx_store4(p, n, m, v);
+}
+
 template <int RG, int NT>
-static void launch_tile(const MxParams & p, bool xf32, hipStream_t s) {
-    const dim3 grid((unsigned) ((p.M + RG * 32 - 1) / (RG * 32)), (unsigned) ((p.N + NT * 64 - 1) / (NT * 64)), 1);
-    if (xf32) hipLaunchKernelGGL((mx_tile<RG, NT, true>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((mx_tile<RG, NT, false>), grid, dim3(512), 0, s, p);
+static void launch_few(const MxParams & p, bool xf32, int splits, hipStream_t s) {
+    const dim3 grid((unsigned) ((p.M + 16 * RG - 1) / (16 * RG)), (unsigned) ((p.N + 16 * NT - 1) / (16 * NT)),
+                    (unsigned) splits);
+    // f32 rows of two token tiles at most are rounded on the way.
+    if constexpr (NT <= 2)
+        if (xf32) {
+            hipLaunchKernelGGL((mx_few<RG, NT, true>), grid, dim3(kMxWaves * 64), 0, s, p);
+            return;
+        }
+    hipLaunchKernelGGL((mx_few<RG, NT, false>), grid, dim3(kMxWaves * 64), 0, s, p);
+}
+template <int NT>
+static void launch_few_rows(const MxParams & p, bool xf32, int rg, int splits, hipStream_t s) {
+    if (rg == 1) launch_few<1, NT>(p, xf32, splits, s);
+    else if (rg == 2) launch_few<2, NT>(p, xf32, splits, s);
+    else launch_few<4, NT>(p, xf32, splits, s);
+}
+
+template <int RG, int NT, int WM, int WN>
+static void launch_tile(const MxParams & p, int splits, hipStream_t s) {
+    constexpr int BM = RG * 16 * WM, BN = NT * 16 * WN;
+    const dim3 grid((unsigned) ((p.M + BM - 1) / BM), (unsigned) ((p.N + BN - 1) / BN), (unsigned) splits);
+    hipLaunchKernelGGL((mx_tile<RG, NT, WM, WN>), grid, dim3(64 * WM * WN), 0, s, p);
+}
+
+// A plan for the tiles: the variant and K splits of the least modelled time
+// (us, 256 CUs).  A step of 128 values of c workgroups on a CU takes `base` +
+// c * `more` (measured: 224 x 256 tiles 3.4 each, 128 x 256 2.2 each, 128 x 128
+// 1.4 alone and 2.5 in pairs, 64 x 64 0.69 and 1.03); the planes of the splits
+// are written and read at 5 TB/s and cost one more launch.  Modelled and
+// measured: 14336 x 128 x 4096 in 128 x 128 tiles and 2 splits 35.3 and 35.3,
+// 4096 x 128 x 4096 in 64 x 64 and 4 splits 18.6 and 20.5 (128 x 128 in 4:
+// 21.6 and 23.5, 64 x 64 unsplit: 26 and 29).
+struct TilePlan {
+    int kind, splits;
+};
+static TilePlan tile_plan(int64_t M, int64_t N, int steps, size_t ws_bytes) {
+    static const struct {
+        int bm, bn;
+        double base, more;
+    } kinds[] = {{224, 256, 0, 3.4}, {128, 256, 0, 2.2}, {128, 128, 0.3, 1.1}, {64, 64, 0.35, 0.34}};
+    TilePlan best{2, 1};
+    double least = 0;
+    for (int k = 0; k < 4; ++k)
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            const double planes = (double) splits * (double) N * (double) M * 4;
+            if (splits > 1 && (steps / splits < 4 || planes > (double) ws_bytes)) break;
+            const int64_t tiles = ((M + kinds[k].bm - 1) / kinds[k].bm) * ((N + kinds[k].bn - 1) / kinds[k].bn);
+            const double c = (double) ((tiles * splits + 255) / 256);
+            const double t = (steps + splits - 1) / splits * (kinds[k].base + c * kinds[k].more) +
+                             (splits > 1 ? 3 + 2 * planes / 5e6 : 0);
+            if (least == 0 || t < least) {
+                least = t;
+                best = {k, splits};
+            }
+        }
+    return best;
+}
+
+// One product with bf16 activations, or f32 ones for at most 32 tokens.
+static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipStream_t s) {
+    const int steps = (p.kb + 3) / 4;
+    const int64_t groups = (p.M + 15) / 16;
+    // Few tokens: row groups to a wave while that leaves 200 workgroups (x is
+    // read once a workgroup; 14336 x 48 x 4096 with 4, 2 and 1 groups: 20, 24
+    // and 36 us, 4096 x 48 x 4096 with 1 and 2: 10.6 and 13).  49 to 64 tokens
+    // on that many rows go to the tiles (14336 x 64 x 4096: 29 us here).
+    const bool near = std::max(p.ws, p.ldx * 2) < (1ll << 23);  // a tile's 256 rows within 32-bit offsets
+    const bool few = p.N <= 48 || (p.N <= 64 && groups < 400) || !near;
+    int rg = groups >= 800 ? 4 : groups >= 400 ? 2 : 1, splits = 1;
+    TilePlan plan{};
+    if (!few) {
+        plan = tile_plan(p.M, p.N, steps, ws_bytes);
+        splits = plan.splits;
+    } else if (p.N > 32 && steps >= 96 && groups <= 256 && 16 * (size_t) p.N * (size_t) p.M <= ws_bytes) {
+        // Long rows, few of them: four K splits of 256 workgroups in all
+        // (2048 x 64 x 14336: 18 us against 26, 4096 x 48 x 14336: 22 against 28).
+        splits = 4;
+        rg = groups > 128 ? 4 : groups > 64 ? 2 : 1;
+    }
+    p.steps = (steps + splits - 1) / splits;
+    splits = (steps + p.steps - 1) / p.steps;
+    const MxParams whole = p;
+    if (splits > 1) {
+        p.y = ws;
+        p.y_f32 = 1;
+        p.ldy = p.M;
+        p.epi = WAMX_EPI_NONE;
+        p.plane = p.N * p.M * 4;
+    }
+    if (few) {
+        if (p.N <= 16) launch_few_rows<1>(p, xf32, rg, splits, s);
+        else if (p.N <= 32) launch_few_rows<2>(p, xf32, rg, splits, s);
+        else if (p.N <= 48) launch_few_rows<3>(p, xf32, rg, splits, s);
+        else if (rg == 1) launch_few<1, 4>(p, xf32, splits, s);
+        else launch_few<2, 4>(p, xf32, splits, s);
+    } else if (plan.kind == 0) {
+        launch_tile<7, 4, 2, 4>(p, splits, s);
+    } else if (plan.kind == 1) {
+        launch_tile<4, 4, 2, 4>(p, splits, s);
+    } else if (plan.kind == 2) {
+        launch_tile<4, 2, 2, 4>(p, splits, s);
+    } else {
+        launch_tile<2, 2, 2, 2>(p, splits, s);
+    }
+    if (splits > 1)
+        hipLaunchKernelGGL(mx_reduce, dim3((unsigned) ((p.N * ((p.M + 3) / 4) + 255) / 256)), dim3(256), 0, s, whole,
+                           (const float *) ws, splits);
 }
 
 hipError_t launch_mx_quantize(const void * x, int32_t x_type, int64_t ldx, void * q, int64_t rows, int64_t cols,
@@ -640,11 +814,27 @@ hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     p.epi = a.epi;
     p.steps = (p.kb + 3) / 4;
     const bool xf32 = a.x_type == WAMX_TYPE_F32;
-    if (a.N <= 16) launch_few<1, 1>(p, xf32, s);
-    else if (a.N <= 32) launch_few<1, 2>(p, xf32, s);
-    else if (a.N <= 64) launch_few<2, 4>(p, xf32, s);
-    else if (a.N <= 600) launch_tile<4, 2>(p, xf32, s);
-    else launch_tile<8, 4>(p, xf32, s);
+    // Tokens in parts that a grid takes.  f32 activations of more than 32: rounded
+    // once into half of the workspace, as many rows at a time as it holds.
+    const bool round = xf32 && a.N > 32;
+    const size_t row = (size_t) a.K * 2, half = a.ws ? a.ws_bytes / 2 : 0;
+    int64_t part = 1 << 20;
+    if (round) part = std::min<int64_t>(std::min<int64_t>(part, (int64_t) (half / row)), 0x3fffffff / (a.K / 8) * 256);
+    if (part < 1) return hipErrorInvalidValue;
+    for (int64_t n = 0; n < a.N; n += part) {
+        MxParams q = p;
+        q.N = std::min(part, a.N - n);
+        q.x = (const char *) p.x + n * p.ldx * (xf32 ? 4 : 2);
+        q.y = (char *) p.y + n * p.ldy * (p.y_f32 ? 4 : 2);
+        q.res = p.res ? p.res + n * p.ldres : nullptr;
+        if (round) {
+            hipLaunchKernelGGL(mx_round_rows, dim3((unsigned) ((q.N * (a.K / 8) + 255) / 256)), dim3(256), 0, s,
+                               (const float *) q.x, a.ldx, (uint16_t *) a.ws, q.N, (int) (a.K / 8));
+            q.x = a.ws;
+            q.ldx = a.K;
+        }
+        run_product(q, xf32 && !round, (char *) a.ws + (round ? half : 0), round ? half : a.ws_bytes, s);
+    }
     return hipGetLastError();
 }
 
