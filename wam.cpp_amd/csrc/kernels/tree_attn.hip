@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace wamx {
 
@@ -40,33 +41,48 @@ constexpr int kTreeWaves = 4, kTreeMax = 256, kTreeWords = kTreeMax / 32;
 
 // The path of every token as a bit set, by doubling: after round r a token
 // holds the 2^r nearest of its ancestors, and its jump leads past them.  A
-// parent outside [-1, tq) marks a slot without a token.
-struct TreePaths {
-    uint32_t bits[2][kTreeMax][kTreeWords];
+// parent outside [-1, tq) marks a slot without a token.  `work` is LDS that the
+// workgroup uses for something else afterwards (a barrier ends this).
+struct TreeWork {
+    uint32_t bits[kTreeMax][kTreeWords];
     int16_t jump[2][kTreeMax];
 };
-__device__ __forceinline__ const uint32_t (*tree_paths(TreePaths & s, const int32_t * parents, int tq))[kTreeWords] {
+typedef uint32_t TreePaths[kTreeMax][kTreeWords];
+__device__ __forceinline__ void tree_paths(TreePaths & path, void * work, const int32_t * parents, int tq) {
+    TreeWork & w = *(TreeWork *) work;
     const int words = (tq + 31) / 32;
+    int rounds = 0;
+    while ((1 << rounds) < tq) ++rounds;
+    // The last round writes `path`.
+    uint32_t (*from)[kTreeWords] = rounds & 1 ? w.bits : path;
+    uint32_t (*to)[kTreeWords] = rounds & 1 ? path : w.bits;
     for (int i = threadIdx.x; i < tq; i += blockDim.x) {
         const int pr = parents[i];
-        s.jump[0][i] = (int16_t) (pr >= 0 && pr < tq ? pr : -1);
+        w.jump[0][i] = (int16_t) (pr >= 0 && pr < tq ? pr : -1);
         const bool token = pr >= -1 && pr < tq;
-        for (int w = 0; w < words; ++w) s.bits[0][i][w] = token && w == i / 32 ? 1u << (i & 31) : 0u;
+        for (int k = 0; k < words; ++k) from[i][k] = token && k == i / 32 ? 1u << (i & 31) : 0u;
     }
     __syncthreads();
-    int cur = 0;
-    for (int span = 1; span < tq; span *= 2, cur ^= 1) {
+    for (int r = 0; r < rounds; ++r) {
         for (int i = threadIdx.x; i < tq; i += blockDim.x) {
-            const int j = s.jump[cur][i];
-            s.jump[cur ^ 1][i] = j >= 0 ? s.jump[cur][j] : (int16_t) -1;
-            for (int w = 0; w < words; ++w) s.bits[cur ^ 1][i][w] = s.bits[cur][i][w] | (j >= 0 ? s.bits[cur][j][w] : 0u);
+            const int j = w.jump[r & 1][i];
+            w.jump[(r & 1) ^ 1][i] = j >= 0 ? w.jump[r & 1][j] : (int16_t) -1;
+            for (int k = 0; k < words; ++k) to[i][k] = from[i][k] | (j >= 0 ? from[j][k] : 0u);
         }
         __syncthreads();
+        uint32_t (*t)[kTreeWords] = from;
+        from = to;
+        to = t;
     }
-    return s.bits[cur];
 }
 
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
+
+// The offset that a row's exponents are taken from: its first maximum, raised
+// only when a tile's passes it by more than 2^8, so that the sums are seldom
+// rescaled (16 rows of a wave see some new maximum in half of all tiles).  A
+// weight is then at most 2^8, as exact in bf16 as one below 1.
+__device__ __forceinline__ float tree_offset(float m, float top) { return top > m + 8.0f || m == -INFINITY ? top : m; }
 
 // Eight values of Q with the scale's sign.
 __device__ __forceinline__ bf16x8_t tree_q(const TreeParams & p, const uint16_t * q) {
@@ -179,7 +195,8 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
     __shared__ __align__(16) uint16_t qs[R * DH];
     __shared__ __align__(16) uint16_t ps[R * TILE];
     __shared__ float sm[kTreeWaves][R];
-    __shared__ TreePaths paths;
+    __shared__ TreePaths path;
+    __shared__ TreeWork work;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
@@ -231,8 +248,7 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
     int tok[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) tok[i] = min(row0 + i * 16 + c16, rows - 1) % p.tq;
-    const uint32_t (*path)[kTreeWords] = paths.bits[0];
-    if (t0 < t1 && t1 * TILE > past) path = tree_paths(paths, parents, p.tq);
+    if (t0 < t1 && t1 * TILE > past) tree_paths(path, &work, parents, p.tq);
     __syncthreads();
 
     float m[NR], l[NR];
@@ -285,7 +301,7 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             const int r = i * 16 + c16;
-            const float mn = fmaxf(fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])), m[i]);
+            const float mn = tree_offset(m[i], fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
             const float bm = mn == -INFINITY ? 0.0f : mn;
             const float alpha = __builtin_amdgcn_exp2f(m[i] - bm);
             float pr[4], sum = 0.0f;
@@ -399,12 +415,13 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
 // as it stands.  K and V^T tiles of 64 slots go through registers into one of
 // two LDS buffers while the other is used; one barrier a tile.
 template <int DH, int NR, int W>
-__global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
+__global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 16, TILE = 64, R = W * NR * 16, QCH = DH / 8;
     constexpr int KN = TILE * QCH / (W * 64), VN = DH * 8 / (W * 64);  // 16-byte pieces of a thread
     __shared__ __align__(16) uint16_t kt_lds[2][TILE * DH];
     __shared__ __align__(16) uint16_t vt_lds[2][DH * TILE];
-    __shared__ TreePaths paths;
+    __shared__ TreePaths path;
+    static_assert(sizeof(TreeWork) <= sizeof vt_lds, "the paths' scratch lies in the value tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
@@ -430,32 +447,39 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
     auto kswz = [](int k) {
         return DH == 64 ? ((k >> 1) & 1) | ((k >> 3) & 3) << 1 : (k & 3) | ((k >> 3) & 3) << 2;
     };
-    bf16x8_t kr[KN], vr[VN];
-    auto request = [&](int64_t kt) {
+    // K of the next tile is requested before this tile's scores and deposited
+    // after them, V then, behind the softmax and the products.
+    static_assert(KN == VN, "one set of registers for both");
+    bf16x8_t sr[KN];
+    auto request_k = [&](int64_t kt) {
 #pragma unroll
         for (int j = 0; j < KN; ++j) {
             const int e = threadIdx.x + j * W * 64;
-            kr[j] = *(const bf16x8_t *) (kb + min(kt * TILE + e / QCH, n - 1) * DH + e % QCH * 8);
+            sr[j] = *(const bf16x8_t *) (kb + min(kt * TILE + e / QCH, n - 1) * DH + e % QCH * 8);
         }
+    };
+    auto request_v = [&](int64_t kt) {
 #pragma unroll
         for (int j = 0; j < VN; ++j) {
             const int e = threadIdx.x + j * W * 64;
-            vr[j] = *(const bf16x8_t *) (vb + (int64_t) (e >> 3) * p.vt_ld + min(kt * TILE + (e & 7) * 8, p.vt_ld - 8));
+            sr[j] = *(const bf16x8_t *) (vb + (int64_t) (e >> 3) * p.vt_ld + min(kt * TILE + (e & 7) * 8, p.vt_ld - 8));
         }
     };
-    auto deposit = [&](int buf) {
+    auto deposit_k = [&](int buf) {
 #pragma unroll
         for (int j = 0; j < KN; ++j) {
             const int e = threadIdx.x + j * W * 64, k = e / QCH;
-            *(bf16x8_t *) (kt_lds[buf] + k * DH + ((e % QCH) ^ kswz(k)) * 8) = kr[j];
+            *(bf16x8_t *) (kt_lds[buf] + k * DH + ((e % QCH) ^ kswz(k)) * 8) = sr[j];
         }
+    };
+    auto deposit_v = [&](int buf) {
 #pragma unroll
         for (int j = 0; j < VN; ++j) {
             const int e = threadIdx.x + j * W * 64, d = e >> 3;
-            *(bf16x8_t *) (vt_lds[buf] + d * TILE + ((e & 7) ^ ((d >> 1) & 7)) * 8) = vr[j];
+            *(bf16x8_t *) (vt_lds[buf] + d * TILE + ((e & 7) ^ ((d >> 1) & 7)) * 8) = sr[j];
         }
     };
-    if (t0 < t1) request(t0);
+    if (t0 < t1) request_k(t0);
     int tok[NR];
     bf16x8_t qf[NR][KC];
 #pragma unroll
@@ -466,9 +490,12 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
 #pragma unroll
         for (int c = 0; c < KC; ++c) qf[i][c] = tree_q(p, qr + c * 32 + g * 8);
     }
-    const uint32_t (*path)[kTreeWords] = paths.bits[0];
-    if (t0 < t1 && t1 * TILE > past) path = tree_paths(paths, parents, p.tq);
-    if (t0 < t1) deposit(0);
+    if (t0 < t1 && t1 * TILE > past) tree_paths(path, vt_lds, parents, p.tq);
+    if (t0 < t1) {
+        deposit_k(0);
+        request_v(t0);
+        deposit_v(0);
+    }
     __syncthreads();
 
     float m[NR], l[NR];
@@ -481,13 +508,14 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
         for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0, 0, 0, 0};
     }
     bool bad = false;
-    for (int64_t kt = t0; kt < t1; ++kt) {
+    // EDGE: a tile that reaches past the cache, where every slot is looked at.
+    auto tile = [&](int64_t kt, auto edge_tag) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(edge_tag)::value;
         const int buf = (int) (kt - t0) & 1;
         const int64_t base = kt * TILE;
-        const bool edge = base + TILE > past;
-        if (kt + 1 < t1) request(kt + 1);
+        if (kt + 1 < t1) request_k(kt + 1);
+        f32x4_t s[NR][4];
         if (row0 < rows) {
-            f32x4_t s[NR][4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int k = (u >> 1) * 32 + 8 * (c16 >> 2) + 4 * (u & 1) + (c16 & 3);
@@ -501,6 +529,12 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
                         s[i][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][c], s[i][u], 0, 0, 0);
                 }
             }
+        }
+        if (kt + 1 < t1) {
+            deposit_k(buf ^ 1);
+            request_v(kt + 1);
+        }
+        if (row0 < rows) {
             bf16x8_t pf[NR][2];
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
@@ -523,7 +557,7 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
                         top = fmaxf(top, v);
                     }
                 top = max_xor32(max_xor16(top)) * p.scale;
-                const float mn = fmaxf(m[i], top);
+                const float mn = tree_offset(m[i], top);
                 const float bm = mn == -INFINITY ? 0.0f : mn;
                 const float alpha = __builtin_amdgcn_exp2f(m[i] - bm);
                 float sum = 0.0f;
@@ -569,9 +603,12 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
                         o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, pf[i][h], o[i][d], 0, 0, 0);
                 }
         }
-        if (kt + 1 < t1) deposit(buf ^ 1);
+        if (kt + 1 < t1) deposit_v(buf ^ 1);
         lds_barrier();
-    }
+    };
+    const int64_t inner = max(t0, min(t1, past / TILE));
+    for (int64_t kt = t0; kt < inner; ++kt) tile(kt, std::false_type{});
+    for (int64_t kt = inner; kt < t1; ++kt) tile(kt, std::true_type{});
     if (__any(bad)) {
         // Inf or NaN among the drafted values: added element by element to the
         // rows whose path holds the slot.
@@ -619,49 +656,83 @@ __global__ __launch_bounds__(W * 64) void tree_attn_many(TreeParams p) {
     }
 }
 
-// out = sum_s po_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): a workgroup per row, its
-// threads DH / 4 pieces of four values by 1024 / DH groups of splits, whose
-// sums are added in order.
-template <int DH>
-__global__ __launch_bounds__(256) void tree_attn_join(TreeParams p) {
-    constexpr int PC = DH / 4, GR = 256 / PC;
+// out = sum_s po_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over a row's units, DH / 4
+// threads with four values each.  BY_ROWS: 1024 / DH rows of one (sequence, key
+// head) to a workgroup, each thread over all units (many rows of few units);
+// else one row, its units shared out among as many groups of threads, whose
+// results are added in order.
+template <int DH, bool BY_ROWS>
+__global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int row_parts) {
+    constexpr int PC = DH / 4, GR = 256 / PC, AT_ONCE = 8;
     __shared__ __align__(16) f32x4_t acc[GR][PC];
-    __shared__ float part[GR];
+    __shared__ float parts[GR][2];
     const int piece = threadIdx.x % PC, gr = threadIdx.x / PC;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
-    const uint32_t bz = blockIdx.x / (uint32_t) rows;
-    const int row = (int) (blockIdx.x - bz * (uint32_t) rows);
+    const uint32_t bz = blockIdx.x / (uint32_t) row_parts;
+    const int first = (int) (blockIdx.x - bz * (uint32_t) row_parts) * (BY_ROWS ? GR : 1);
+    const int row = min(first + (BY_ROWS ? gr : 0), rows - 1);
     const int64_t b = bz / (uint32_t) p.kv_heads;
     const int hk = (int) (bz - (uint32_t) b * (uint32_t) p.kv_heads);
     const TreeUnit unit = tree_unit(p, 0, (int) b);
     const int64_t step = (int64_t) p.kv_heads * rows, at = unit.first * step + hk * rows + row;
-    float m = -INFINITY;
-    for (int s = threadIdx.x & 63; s < unit.count; s += 64) m = fmaxf(m, p.pml[2 * (at + s * step)]);
-    m = wave_max(m);
-    const float bm = m == -INFINITY ? 0.0f : m;
+    float m = -INFINITY, sum = 0.0f;
     f32x4_t v = {0, 0, 0, 0};
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int s = gr; s < unit.count; s += GR) {
-        const float f = __builtin_amdgcn_exp2f(p.pml[2 * (at + s * step)] - bm);
-        const f32x4_t o = *(const f32x4_t *) (p.po + (at + s * step) * DH + piece * 4);
-        sum += p.pml[2 * (at + s * step) + 1] * f;
-        // A unit without a slot of this row (f = 0) holds zeros.
-        v += o * f;
-    }
-    acc[gr][piece] = v;
-    if (piece == 0) part[gr] = sum;
-    __syncthreads();
-    if (gr) return;
-    sum = part[0];
+    constexpr int BY = BY_ROWS ? 1 : GR;
+    for (int s0 = BY_ROWS ? 0 : gr; s0 < unit.count; s0 += AT_ONCE * BY) {
+        float ms[AT_ONCE], ls[AT_ONCE];
+        f32x4_t o[AT_ONCE];
 #pragma unroll
-    for (int k = 1; k < GR; ++k) {
-        v += acc[k][piece];
-        sum += part[k];
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int64_t j = at + min(s0 + k * BY, unit.count - 1) * step;
+            const float2 ml = *(const float2 *) (p.pml + 2 * j);
+            ms[k] = s0 + k * BY < unit.count ? ml.x : -INFINITY;
+            ls[k] = ml.y;
+            o[k] = *(const f32x4_t *) (p.po + j * DH + piece * 4);
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ms[k]);
+        const float bm = top == -INFINITY ? 0.0f : top, old = __builtin_amdgcn_exp2f(m - bm);
+        sum *= old;
+        v *= old;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            // A unit without a slot of this row has no part (it may hold NaN).
+            if (ms[k] == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(ms[k] - bm);
+            sum += ls[k] * f;
+            v += o[k] * f;
+        }
     }
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
-    uint16_t * y = p.out + ((b * p.tq + row % p.tq) * p.heads + hk * group + row / p.tq) * DH + piece * 4;
+    if constexpr (!BY_ROWS) {
+        acc[gr][piece] = v;
+        if (piece == 0) {
+            parts[gr][0] = m;
+            parts[gr][1] = sum;
+        }
+        __syncthreads();
+        if (gr) return;
+        float top = m;
+#pragma unroll
+        for (int k = 1; k < GR; ++k) top = fmaxf(top, parts[k][0]);
+        const float bm = top == -INFINITY ? 0.0f : top;
+        const float old = __builtin_amdgcn_exp2f(m - bm);
+        v *= old;
+        sum *= old;
+#pragma unroll
+        for (int k = 1; k < GR; ++k) {
+            const float f = __builtin_amdgcn_exp2f(parts[k][0] - bm);
+            v += acc[k][piece] * f;
+            sum += parts[k][1] * f;
+        }
+        m = top;
+    } else if (first + gr >= rows) {
+        return;
+    }
     const bool none = m == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / sum;
+    uint16_t * y = p.out + ((b * p.tq + row % p.tq) * p.heads + hk * group + row / p.tq) * DH + piece * 4;
     *(uint32_t *) y = none ? 0u : pack_bf16x2(v[0] * inv, v[1] * inv);
     *(uint32_t *) (y + 2) = none ? 0u : pack_bf16x2(v[2] * inv, v[3] * inv);
 }
@@ -690,7 +761,17 @@ static hipError_t launch(void (*kernel)(TreeParams), int R, int threads, int64_t
     const int64_t wgs = ((int64_t) p.units * a.kv_heads + 7) / 8 * 8 * rt, joins = a.batch * a.kv_heads * rows;
     if (wgs > 0x7fffffff || joins > 0x7fffffff) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kernel, dim3((unsigned) wgs), dim3((unsigned) threads), 0, s, p);
-    if (p.po) hipLaunchKernelGGL(tree_attn_join<DH>, dim3((unsigned) joins), dim3(256), 0, s, p);
+    if (p.po) {
+        // Many rows have few units each (64 tokens of 4 x 8 heads, 8 units: a
+        // workgroup per row 16.6 us), few rows many.
+        if (p.units <= 16 * a.batch) {
+            const int parts = (int) ((rows + 1024 / DH - 1) / (1024 / DH));
+            hipLaunchKernelGGL((tree_attn_join<DH, true>), dim3((unsigned) (a.batch * a.kv_heads * parts)), dim3(256), 0, s,
+                               p, parts);
+        } else {
+            hipLaunchKernelGGL((tree_attn_join<DH, false>), dim3((unsigned) joins), dim3(256), 0, s, p, (int) rows);
+        }
+    }
     return hipGetLastError();
 }
 
