@@ -48,7 +48,7 @@ struct TreeWork {
     int16_t jump[2][kTreeMax];
 };
 typedef uint32_t TreePaths[kTreeMax][kTreeWords];
-__device__ __forceinline__ void tree_paths(TreePaths & path, void * work, const int32_t * parents, int tq) {
+__device__ __forceinline__ void tree_paths(TreePaths & path, void * work, int parent, int tq) {
     TreeWork & w = *(TreeWork *) work;
     const int words = (tq + 31) / 32;
     int rounds = 0;
@@ -56,15 +56,15 @@ __device__ __forceinline__ void tree_paths(TreePaths & path, void * work, const 
     // The last round writes `path`.
     uint32_t (*from)[kTreeWords] = rounds & 1 ? w.bits : path;
     uint32_t (*to)[kTreeWords] = rounds & 1 ? path : w.bits;
-    for (int i = threadIdx.x; i < tq; i += blockDim.x) {
-        const int pr = parents[i];
-        w.jump[0][i] = (int16_t) (pr >= 0 && pr < tq ? pr : -1);
-        const bool token = pr >= -1 && pr < tq;
+    const int i = threadIdx.x;
+    if (i < tq) {
+        w.jump[0][i] = (int16_t) (parent >= 0 && parent < tq ? parent : -1);
+        const bool token = parent >= -1 && parent < tq;
         for (int k = 0; k < words; ++k) from[i][k] = token && k == i / 32 ? 1u << (i & 31) : 0u;
     }
     __syncthreads();
     for (int r = 0; r < rounds; ++r) {
-        for (int i = threadIdx.x; i < tq; i += blockDim.x) {
+        if (i < tq) {
             const int j = w.jump[r & 1][i];
             w.jump[(r & 1) ^ 1][i] = j >= 0 ? w.jump[r & 1][j] : (int16_t) -1;
             for (int k = 0; k < words; ++k) to[i][k] = from[i][k] | (j >= 0 ? from[j][k] : 0u);
@@ -107,29 +107,46 @@ __device__ float tree_weight(const TreeParams & p, int64_t b, int64_t head, int6
     return __builtin_amdgcn_exp2f(s * p.scale - m);
 }
 
+// Which of 32 slots a token sees, the first being drafted slot `off` (negative:
+// still in the cache, where every slot is seen).
+__device__ __forceinline__ uint32_t tree_seen(const uint32_t * path, int64_t off, int tq) {
+    if (off <= -32) return 0xffffffffu;
+    const int o = off < tq ? (int) off : kTreeMax, words = (tq + 31) / 32, w = o >> 5, sh = o & 31;
+    const uint32_t lo = w < 0 ? 0xffffffffu : w < words ? path[w] : 0u, hi = w + 1 < words ? path[w + 1] : 0u;
+    return sh ? lo >> sh | hi << (32 - sh) : lo;
+}
+
 // Eight values of V^T from `slot` on in a tile that reaches past `past`: slots
 // behind the last hold anything and become zero, and so do Inf and NaN of a
 // drafted slot, which must not reach the rows that do not see it (true: there
 // is one, added to the rows that do by itself).
 __device__ __forceinline__ bool tree_mask_values(uint32_t * w, int64_t slot, int64_t past, int64_t n) {
+    const int held = (int) max((int64_t) 0, min((int64_t) 8, n - slot));
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        w[j] &= held > 2 * j + 1 ? 0xffffffffu : held == 2 * j + 1 ? 0x0000ffffu : 0u;
+        any |= not_finite_bf16(w[j]) || not_finite_bf16(w[j] >> 16);
+    }
+    if (!any || slot + 8 <= past) return false;
     bool bad = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const bool odd = slot + j >= past && slot + j < n && not_finite_bf16(w[j >> 1] >> (16 * (j & 1)));
-        bad |= odd;
-        if (odd || slot + j >= n) w[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-    }
+    for (int j = 0; j < 8; ++j)
+        if (slot + j >= past && not_finite_bf16(w[j >> 1] >> (16 * (j & 1)))) {
+            bad = true;
+            w[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
     return bad;
 }
 
 // The units of the slots: sequence b gets 1 + (units - batch) tiles_b / tiles of
-// them (its share by length, but four tiles a unit at least), one after another;
+// them (its share by length, but kTreeLeast tiles a unit at least), one after another;
 // units / batch each where the sequences are more than a wave's lanes (or the
 // product would pass 32 bits).  Unit u's sequence, the first of that sequence's
 // units and their number; no sequence (-1) past the last unit.
-constexpr int kTreeTile = 64;
+constexpr int kTreeTile = 64, kTreeLeast = 2;
 struct TreeUnit {
-    int b, first, count;
+    int b, first, count, slots;
 };
 __device__ __forceinline__ int64_t tree_slots(const TreeParams & p, int b) {
     // A length that does not fit leaves its sequence without slots.
@@ -140,17 +157,18 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams & p, int u, int b
     if (p.even) {
         const int each = (int) ((uint32_t) p.units / (uint32_t) p.batch);
         const int b = b_known >= 0 ? b_known : (int) ((uint32_t) u / (uint32_t) each);
-        return {b < p.batch ? b : -1, b * each, each};
+        return {b < p.batch ? b : -1, b * each, each, b < p.batch ? (int) tree_slots(p, b) : 0};
     }
     const int lane = threadIdx.x & 63;
-    const uint32_t tiles = lane < p.batch ? (uint32_t) ((tree_slots(p, lane) + kTreeTile - 1) / kTreeTile) : 0;
+    const int slots = lane < p.batch ? (int) tree_slots(p, lane) : 0;
+    const uint32_t tiles = ((uint32_t) slots + kTreeTile - 1) / kTreeTile;
     uint32_t sum = tiles;
     for (int o = 1; o < p.batch; o <<= 1) sum += (uint32_t) __shfl_xor((int) sum, o);
     // Past the batch's power of two the lanes hold nothing, and take nothing.
     int mine = 0;
     if (lane < p.batch) {
         mine = 1 + (sum ? (int) ((uint32_t) (p.units - p.batch) * tiles / sum) : 0);
-        mine = min(mine, max(1, (int) (tiles / 4)));
+        mine = min(mine, max(1, (int) (tiles / kTreeLeast)));
     }
     int end = mine;  // inclusive prefix
     for (int o = 1; o < p.batch; o <<= 1) {
@@ -160,11 +178,11 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams & p, int u, int b
     int b = b_known;
     if (b < 0) {
         const unsigned long long past_u = __ballot(lane < p.batch && end > u);
-        if (!past_u) return {-1, 0, 0};
+        if (!past_u) return {-1, 0, 0, 0};
         b = __ffsll(past_u) - 1;
     }
     const int count = __shfl(mine, b);
-    return {b, __shfl(end, b) - count, count};
+    return {b, __shfl(end, b) - count, count, __shfl(slots, b)};
 }
 // The tiles [t0, t1) of part i out of `count`.
 __device__ __forceinline__ void tree_range(int64_t n, int i, int count, int64_t & t0, int64_t & t1) {
@@ -190,7 +208,7 @@ __device__ __forceinline__ void lds_barrier() {
 // and the probabilities lie in LDS.  K of the next tile is requested when this
 // tile's scores are done and V when its product is.
 template <int DH, int NR>
-__global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) {
+__global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 64, TILE = 64, R = NR * 16, QCH = DH / 8;
     __shared__ __align__(16) uint16_t qs[R * DH];
     __shared__ __align__(16) uint16_t ps[R * TILE];
@@ -210,11 +228,12 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
     const TreeUnit unit = tree_unit(p, u);
     if (unit.b < 0) return;
     const int b = unit.b;
-    const int64_t n = tree_slots(p, b), past = n ? n - p.tq : 0;
+    const int64_t n = unit.slots, past = n ? n - p.tq : 0;
     int64_t t0, t1;
     tree_range(n, u - unit.first, unit.count, t0, t1);
     const int64_t bz = (int64_t) b * p.kv_heads + hk;
     const int32_t * parents = p.parents + (int64_t) b * p.tq;
+    const int parent = (int) threadIdx.x < p.tq ? parents[threadIdx.x] : -1;
 
     const uint16_t * kb = p.k + bz * p.capacity * DH + g * 8;
     const uint16_t * vb = p.vt + (bz * DH + wave * (DH / 4) + c16) * p.vt_ld;
@@ -246,9 +265,14 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
         *(bf16x8_t *) (qs + r * DH + (c ^ qswz(r)) * 8) = tree_q(p, qr + c * 8);
     }
     int tok[NR];
+    bool token[NR];  // a place that holds a token
 #pragma unroll
-    for (int i = 0; i < NR; ++i) tok[i] = min(row0 + i * 16 + c16, rows - 1) % p.tq;
-    if (t0 < t1 && t1 * TILE > past) tree_paths(path, &work, parents, p.tq);
+    for (int i = 0; i < NR; ++i) {
+        tok[i] = min(row0 + i * 16 + c16, rows - 1) % p.tq;
+        const int pr = parents[tok[i]];
+        token[i] = pr >= -1 && pr < p.tq;
+    }
+    if (t0 < t1 && t1 * TILE > past) tree_paths(path, &work, parent, p.tq);
     __syncthreads();
 
     float m[NR], l[NR];
@@ -278,22 +302,12 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
         if (kt + 1 < t1) load_k(kt + 1);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            float top = -INFINITY;
+            if (edge) {
+                const uint32_t seen = tree_seen(path[tok[i]], base + wave * 16 + 4 * g - past, p.tq);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = s[i][r];
-                if (edge) {
-                    const int64_t slot = base + wave * 16 + 4 * g + r;
-                    bool seen = slot < past;
-                    if (slot >= past && slot < n) {
-                        const int a = (int) (slot - past);
-                        seen = path[tok[i]][a >> 5] >> (a & 31) & 1;
-                    }
-                    v = seen ? v : -INFINITY;
-                }
-                s[i][r] = v;
-                top = fmaxf(top, v);
+                for (int r = 0; r < 4; ++r) s[i][r] = seen >> r & 1 ? s[i][r] : -INFINITY;
             }
+            float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
             top = max_xor32(max_xor16(top)) * p.scale;
             if (g == 0) sm[wave][i * 16 + c16] = top;
         }
@@ -383,8 +397,7 @@ __global__ __launch_bounds__(kTreeWaves * 64) void tree_attn_rows(TreeParams p) 
         const int r = i * 16 + c16, row = row0 + r;
         const float sum = (sm[0][r] + sm[1][r]) + (sm[2][r] + sm[3][r]);
         if (row >= rows) continue;
-        const int pr = parents[tok[i]];
-        const bool none = !(pr >= -1 && pr < p.tq) || (sum == 0.0f && m[i] == -INFINITY);
+        const bool none = !token[i] || (sum == 0.0f && m[i] == -INFINITY);
         const int d0 = wave * (DH / 4) + 4 * g;
         if (p.po) {
             const int64_t at = ((int64_t) u * p.kv_heads + hk) * rows + row;
@@ -433,11 +446,12 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
     const TreeUnit unit = tree_unit(p, u);
     if (unit.b < 0) return;
     const int b = unit.b;
-    const int64_t n = tree_slots(p, b), past = n ? n - p.tq : 0;
+    const int64_t n = unit.slots, past = n ? n - p.tq : 0;
     int64_t t0, t1;
     tree_range(n, u - unit.first, unit.count, t0, t1);
     const int64_t bz = (int64_t) b * p.kv_heads + hk;
     const int32_t * parents = p.parents + (int64_t) b * p.tq;
+    const int parent = (int) threadIdx.x < p.tq ? parents[threadIdx.x] : -1;
     const uint16_t * kb = p.k + bz * p.capacity * DH;
     const uint16_t * vb = p.vt + bz * DH * p.vt_ld;
 
@@ -490,7 +504,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
 #pragma unroll
         for (int c = 0; c < KC; ++c) qf[i][c] = tree_q(p, qr + c * 32 + g * 8);
     }
-    if (t0 < t1 && t1 * TILE > past) tree_paths(path, vt_lds, parents, p.tq);
+    if (t0 < t1 && t1 * TILE > past) tree_paths(path, vt_lds, parent, p.tq);
     if (t0 < t1) {
         deposit_k(0);
         request_v(t0);
@@ -538,24 +552,20 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
             bf16x8_t pf[NR][2];
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
+                if (edge) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t seen = tree_seen(path[tok[i]], base + h * 32 + 8 * g - past, p.tq);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            s[i][2 * h + e / 4][e % 4] = seen >> e & 1 ? s[i][2 * h + e / 4][e % 4] : -INFINITY;
+                    }
+                }
                 float top = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float v = s[i][u][r];
-                        if (edge) {
-                            const int64_t slot = base + (u >> 1) * 32 + 8 * g + 4 * (u & 1) + r;
-                            bool seen = slot < past;
-                            if (slot >= past && slot < n) {
-                                const int a = (int) (slot - past);
-                                seen = path[tok[i]][a >> 5] >> (a & 31) & 1;
-                            }
-                            v = seen ? v : -INFINITY;
-                        }
-                        s[i][u][r] = v;
-                        top = fmaxf(top, v);
-                    }
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][u][r]);
                 top = max_xor32(max_xor16(top)) * p.scale;
                 const float mn = tree_offset(m[i], top);
                 const float bm = mn == -INFINITY ? 0.0f : mn;
@@ -737,11 +747,13 @@ __global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int row_part
     *(uint32_t *) (y + 2) = none ? 0u : pack_bf16x2(v[2] * inv, v[3] * inv);
 }
 
-// Units: `wgs` workgroups in all where each has four tiles or more, as far as
-// the workspace holds their results.
+// Units: `wgs` workgroups in all where each has kTreeLeast tiles or more (two:
+// 64 tokens of 4 x 8 heads over 1000 slots 26 us, four tiles 30, one 32; a
+// draft of 8 over 128 slots not split 7.5 us, split 9.7), as far as the
+// workspace holds their results.
 static void plan(TreeParams & p, const TreeArgs & a, int64_t row_tiles, int64_t wgs) {
     const int64_t rows = a.heads / a.kv_heads * a.tq, tiles = (a.capacity + kTreeTile - 1) / kTreeTile;
-    int64_t units = std::min<int64_t>(wgs / (a.kv_heads * row_tiles), a.batch * std::max<int64_t>(tiles / 4, 1));
+    int64_t units = std::min<int64_t>(wgs / (a.kv_heads * row_tiles), a.batch * std::max<int64_t>(tiles / kTreeLeast, 1));
     const size_t per = (size_t) (a.kv_heads * rows) * (size_t) (a.head_dim + 2) * 4;
     if (!a.ws || a.ws_bytes / per < (size_t) units) units = a.ws ? (int64_t) (a.ws_bytes / per) : 0;
     p.even = a.batch > 64 || (uint64_t) units * (uint64_t) tiles * (uint64_t) a.batch > 0xffffffffull;
@@ -775,9 +787,13 @@ static hipError_t launch(void (*kernel)(TreeParams), int R, int threads, int64_t
     return hipGetLastError();
 }
 
+// As many workgroups as it takes to keep 16 MB of slots requested, where the
+// registers let them run together (one token of 4 x 4 heads of 64, 100000 slots:
+// 256 workgroups 62 us, 512 39, 768 36; 8 tokens of 4 x 8 heads of 128: 39, 34,
+// 35; 33 tokens of 8 heads of 256: 35, 37, 39).
 template <int DH, int NR>
 static hipError_t run_rows(TreeParams & p, const TreeArgs & a, hipStream_t s) {
-    return launch<DH>(tree_attn_rows<DH, NR>, NR * 16, kTreeWaves * 64, 768, p, a, s);
+    return launch<DH>(tree_attn_rows<DH, NR>, NR * 16, kTreeWaves * 64, DH == 64 ? 768 : NR * DH == 768 ? 256 : 512, p, a, s);
 }
 template <int DH, int NR, int W>
 static hipError_t run_many(TreeParams & p, const TreeArgs & a, hipStream_t s) {
