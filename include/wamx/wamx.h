@@ -806,7 +806,7 @@ WAMX_API wamx_status  wamx_gguf_get_u64(wamx_gguf_t g, const char * key, uint64_
 WAMX_API wamx_status  wamx_gguf_get_f32(wamx_gguf_t g, const char * key, float * out);
 WAMX_API const char * wamx_gguf_get_str(wamx_gguf_t g, const char * key);
 WAMX_API int64_t      wamx_gguf_get_f32_array(wamx_gguf_t g, const char * key, float * out, int64_t cap);
-/* Tensor descriptors (GgufTensorInfo): name, ggml type (0 F32, 1 F16, 30 BF16,
+/* Tensor descriptors (GgufTensorInfo): name, ggml type (0 F32, 1 F16, 30 BF16, 39 MXFP4,
  * ...), n_dims, ne[dim] (1 past n_dims), absolute file offset, payload bytes
  * (0 for a type this reader does not size).  find returns -1 when absent. */
 WAMX_API int64_t      wamx_gguf_n_tensors(wamx_gguf_t g);

@@ -260,6 +260,9 @@ bool parse(wamx_gguf & g) {
             }
             const int64_t es = type_size(t.type);
             t.bytes = es > 0 ? (uint64_t) n * (uint64_t) es : 0;
+            // MXFP4 (39): 17 bytes for every 32 values of a row.
+            if (t.type == WAMX_TYPE_MXFP4 && t.ne[0] % wamx_blck_size(t.type) == 0)
+                t.bytes = (uint64_t) (n / wamx_blck_size(t.type)) * wamx_type_size(t.type);
             if (t.offset % g.alignment != 0) {
                 g.error = "tensor " + t.name + " data is not aligned";
                 return false;
