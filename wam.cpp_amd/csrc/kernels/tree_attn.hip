@@ -81,8 +81,9 @@ __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80
 // The offset that a row's exponents are taken from: its first maximum, raised
 // only when a tile's passes it by more than 2^8, so that the sums are seldom
 // rescaled (16 rows of a wave see some new maximum in half of all tiles).  A
-// weight is then at most 2^8, as exact in bf16 as one below 1.
-__device__ __forceinline__ float tree_offset(float m, float top) { return top > m + 8.0f || m == -INFINITY ? top : m; }
+// weight is then at most 2^8, as exact in bf16 as one below 1.  A tile whose
+// scores are all NaN leaves it (the sum is NaN then), so it is never NaN itself.
+__device__ __forceinline__ float tree_offset(float m, float top) { return top > m + 8.0f ? top : m; }
 
 // Eight values of Q with the scale's sign.
 __device__ __forceinline__ bf16x8_t tree_q(const TreeParams & p, const uint16_t * q) {
