@@ -57,6 +57,20 @@ def test_rows_further_apart_than_32_bit_offsets(wx, be, N):
     np.testing.assert_array_equal(dy.download(np.float32, (N, M)), xi @ ref.dequantize(w).astype(np.float32).T)
 
 
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+def test_rows_so_far_apart_that_they_go_one_by_one(wx, be, xt):
+    M, N, K, ldx = 40, 5, 96, (1 << 23) + 5
+    rng = np.random.default_rng(7)
+    w = int_weights(rng, M, K)
+    xi = rng.integers(-3, 4, (N, K)).astype(np.float32)
+    xb = np.zeros((N, ldx), np.uint16 if xt == "bf16" else np.float32)
+    xb[:, :K] = wx.f32_to_bf16(xi) if xt == "bf16" else xi
+    dw, dx, dy = be.array(w), be.array(xb), be.empty(N * M * 4)
+    wx.check(be.lib.wamx_op_mul_mat_mxfp4(be.ptr, dw.ptr, dx.ptr, wx.TYPE_BF16 if xt == "bf16" else wx.TYPE_F32, ldx,
+                                          dy.ptr, wx.TYPE_F32, M, M, N, K))
+    np.testing.assert_array_equal(dy.download(np.float32, (N, M)), xi @ ref.dequantize(w).astype(np.float32).T)
+
+
 def test_split_products_replayed_between_other_calls(wx, be):
     """Two computed graphs with split products, replayed in turn with single calls
     that use a workspace too between them."""

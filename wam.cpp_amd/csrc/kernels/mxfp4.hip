@@ -313,7 +313,7 @@ __device__ __forceinline__ bf16x8_t mx_pair(uint32_t lo0, uint32_t lo1, uint32_t
 // steps of 128 in turn (a row's 68 bytes of a step lie next to the next
 // wave's) and their sums meet in LDS in wave order.  Lane (r, g) holds block g
 // of the step for weight row r, and the same 32 values of x for token r.
-constexpr int kMxWaves = 8;
+constexpr int kMxWaves = 8, kMxAhead = 2;
 
 template <int RG, int NT, bool XF32>
 __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
@@ -330,8 +330,9 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
 
     const char * w[RG];
     uint32_t mis[RG];
-    const char * x[NT * 4];
+    uint32_t x[NT * 4];
     constexpr int xs = XF32 ? 4 : 2;
+    const char * xbase = (const char *) p.x + n0 * p.ldx * xs;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
         // Rows of fewer than four blocks: their last one for the lanes past it.
@@ -340,32 +341,36 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
         w[i] -= mis[i];
     }
     // Sixteen lanes read the 256 bytes of a token's step (twice that in f32), a
-    // lane four tokens.
+    // lane four tokens, at 32-bit offsets (launch_mx_product sees to that).
 #pragma unroll
     for (int j = 0; j < NT * 4; ++j)
-        x[j] = (const char *) p.x + (min(n0 + j * 4 + g, p.N - 1) * p.ldx + r * 8) * xs;
+        x[j] = (uint32_t) ((min(n0 + j * 4 + g, p.N - 1) - n0) * p.ldx + r * 8) * xs;
     uint4 * mine = (uint4 *) (lds + wave * XB);
 
-    // The next step is requested when this one's x lies in LDS.
-    MxBlock wr[2][RG];
+    // x of the next step is requested when this one's lies in LDS, the weights
+    // kMxAhead steps before their use (one: 14336 x 48 x 4096 19.1 us for 18.5,
+    // three: spills).
+    MxBlock wr[kMxAhead + 1][RG];
     any16 xr[NT * 4][XF32 ? 2 : 1];
-    auto load = [&](int s, MxBlock * t) {
+    auto load_w = [&](int s, MxBlock * t) {
         // A lane past the row's last block repeats its block of the step before.
         const int64_t o = (int64_t) (s - (s > 0 && 4 * s + g >= p.kb)) * (4 * kMxBytes);
 #pragma unroll
         for (int i = 0; i < RG; ++i) t[i] = mx_load(w[i] + o);
-        const int64_t xo = (4 * s + (r >> 2) < p.kb ? (int64_t) s * 128 : -r * 8) * xs;  // past the row: its start
+    };
+    auto load_x = [&](int s) {
+        const uint32_t xo = (uint32_t) ((4 * s + (r >> 2) < p.kb ? s * 128 : -r * 8) * xs);  // past the row: its start
 #pragma unroll
         for (int j = 0; j < NT * 4; ++j)
 #pragma unroll
-            for (int v = 0; v < (XF32 ? 2 : 1); ++v) xr[j][v] = *(const any16 *) (x[j] + xo + 16 * v);
+            for (int v = 0; v < (XF32 ? 2 : 1); ++v) xr[j][v] = *(const any16 *) (xbase + (x[j] + xo) + 16 * v);
     };
     f32x4_t acc[RG][NT];
 #pragma unroll
     for (int i = 0; i < RG; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
-    auto multiply = [&](int s, int next, MxBlock * t, MxBlock * tn) {
+    auto multiply = [&](int s, int next, int next_w, MxBlock * t, MxBlock * tn) {
         // Through LDS into operand order: piece q of token n in slot q ^ (n % 16),
         // so that the 16 tokens of a read lie in different banks.
         const bool tail = 4 * s + 4 > p.kb;
@@ -396,7 +401,8 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
                 for (int d = 0; d < 4; ++d) t[i].lo.v[d] = 0;
             }
         }
-        if (next >= 0) load(next, tn);
+        if (next >= 0) load_x(next);
+        if (next_w >= 0) load_w(next_w, tn);
         __builtin_amdgcn_wave_barrier();
         // Dwords 2h and 2h + 1 of the codes meet pieces h and h + 2 of block g.
 #pragma unroll
@@ -428,12 +434,17 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
     const int ns = s1 - s0, turn = (int) (blockIdx.x % (uint32_t) ns);
     auto at = [&](int k) { return s0 + (k + turn < ns ? k + turn : k + turn - ns); };
     int k = wave;
-    if (k < ns) load(at(k), wr[0]);
+    if (k < ns) load_x(at(k));
+#pragma unroll
+    for (int d = 0; d < kMxAhead; ++d)
+        if (k + d * kMxWaves < ns) load_w(at(k + d * kMxWaves), wr[d]);
     while (k < ns) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q <= kMxAhead; ++q) {
             if (k >= ns) break;
-            multiply(at(k), k + kMxWaves < ns ? at(k + kMxWaves) : -1, wr[q], wr[q ^ 1]);
+            multiply(at(k), k + kMxWaves < ns ? at(k + kMxWaves) : -1,
+                     k + kMxAhead * kMxWaves < ns ? at(k + kMxAhead * kMxWaves) : -1, wr[q],
+                     wr[(q + kMxAhead) % (kMxAhead + 1)]);
             k += kMxWaves;
         }
     }
@@ -712,13 +723,23 @@ static TilePlan tile_plan(int64_t M, int64_t N, int steps, size_t ws_bytes) {
 static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipStream_t s) {
     const int steps = (p.kb + 3) / 4;
     const int64_t groups = (p.M + 15) / 16;
-    // Few tokens: row groups to a wave while that leaves 200 workgroups (x is
-    // read once a workgroup; 14336 x 48 x 4096 with 4, 2 and 1 groups: 20, 24
-    // and 36 us, 4096 x 48 x 4096 with 1 and 2: 10.6 and 13).  49 to 64 tokens
-    // on that many rows go to the tiles (14336 x 64 x 4096: 29 us here).
+    // Few tokens: groups of 16 rows to a workgroup by how many workgroups a CU
+    // then has to run and what each costs, two for a group's weights and one for
+    // a tile's x (us with 1, 2 and 4 groups: 4096 x 1 x 4096 6.3, 8.0, 12.1;
+    // 20000 x 1 x 4096 21.5, 17.6, 22.7; 14336 x 32 x 4096 24.0, 19.9, 15.7;
+    // 14336 x 48 x 4096 35.8, 24.0, 18.3).  49 to 64 tokens come here while 512
+    // groups, a workgroup per CU, hold the rows (6400 x 64 x 4096 15.2 us, in
+    // tiles 19.9).
     const bool near = std::max(p.ws, p.ldx * 2) < (1ll << 23);  // a tile's 256 rows within 32-bit offsets
-    const bool few = p.N <= 48 || (p.N <= 64 && groups < 400) || !near;
-    int rg = groups >= 800 ? 4 : groups >= 400 ? 2 : 1, splits = 1;
+    const bool few = p.N <= 48 || (p.N <= 64 && groups <= 512) || !near;
+    int rg = 1, splits = 1;
+    int64_t least = 0;
+    for (int c = 1; c <= 4; c *= 2) {
+        const int64_t t = (groups + 256 * c - 1) / (256 * c) * (2 * c + (std::min<int64_t>(p.N, 64) + 15) / 16);
+        if (least && t > least) continue;
+        least = t;
+        rg = c;
+    }
     TilePlan plan{};
     if (!few) {
         plan = tile_plan(p.M, p.N, steps, ws_bytes);
@@ -795,7 +816,7 @@ hipError_t launch_mx_dequantize(const void * q, int64_t qs, const int32_t * rows
 
 hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     if (a.M <= 0 || a.N <= 0) return hipSuccess;
-    if (a.K <= 0 || a.K % 32 != 0 || a.K / 32 > 0x7fffffff) return hipErrorInvalidValue;
+    if (a.K <= 0 || a.K % 32 != 0 || a.K >= 1 << 30) return hipErrorInvalidValue;
     MxParams p{};
     p.w = (const uint8_t *) a.w;
     p.ws = a.w_stride;
@@ -818,7 +839,8 @@ hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     // once into half of the workspace, as many rows at a time as it holds.
     const bool round = xf32 && a.N > 32;
     const size_t row = (size_t) a.K * 2, half = a.ws ? a.ws_bytes / 2 : 0;
-    int64_t part = 1 << 20;
+    // Rows so far apart that 64 of them pass 32-bit offsets go one by one.
+    int64_t part = a.ldx > 1 << 23 ? 1 : 1 << 20;
     if (round) part = std::min<int64_t>(std::min<int64_t>(part, (int64_t) (half / row)), 0x3fffffff / (a.K / 8) * 256);
     if (part < 1) return hipErrorInvalidValue;
     for (int64_t n = 0; n < a.N; n += part) {
