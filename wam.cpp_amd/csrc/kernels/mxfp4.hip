@@ -466,9 +466,10 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
     }
 }
 
-// Many tokens: matrix-core bound.  Eight waves, 2 along the weight rows by 4
-// along the tokens, each RG x NT tiles of 16 x 16 (so RG * 32 rows by NT * 64
-// tokens a workgroup).  The weight stays in its 4 bits down to the register
+// Many tokens: WM waves along the weight rows by WN along the tokens, each RG x
+// NT tiles of 16 x 16.  Every wave expands its rows' codes itself, so 128 x 128
+// tiles take 4 x 2 waves of 2 x 4 tiles (10250 x 333 x 2048: 28.9 us, 2 x 4
+// waves of 4 x 2 tiles 30.5).  The weight stays in its 4 bits down to the register
 // that becomes the operand: a step of 128 values is 4 blocks a row, whose codes
 // lie in LDS as [block][row][g], so that a wave's read of dword g of its rows is
 // 256 bytes in a row.  Such a dword
@@ -688,11 +689,12 @@ static void launch_tile(const MxParams & p, int splits, hipStream_t s) {
 // A plan for the tiles: the variant and K splits of the least modelled time
 // (us, 256 CUs).  A step of 128 values of c workgroups on a CU takes `base` +
 // c * `more` (measured: 224 x 256 tiles 3.4 each, 128 x 256 2.2 each, 128 x 128
-// 1.4 alone and 2.5 in pairs, 64 x 64 0.69 and 1.03); the planes of the splits
-// are written and read at 5 TB/s and cost one more launch.  Modelled and
-// measured: 14336 x 128 x 4096 in 128 x 128 tiles and 2 splits 35.3 and 35.3,
-// 4096 x 128 x 4096 in 64 x 64 and 4 splits 18.6 and 20.5 (128 x 128 in 4:
-// 21.6 and 23.5, 64 x 64 unsplit: 26 and 29).
+// 1.4 alone and 2.4 in pairs, 64 x 64 0.69, 1.03 and with five 2.5); the planes
+// of the splits are written and read at 4 TB/s, and they cost one more launch.
+// Modelled and measured: 14336 x 128 x 4096 in 128 x 128 tiles and 2 splits 35
+// and 34, in 64 x 64 unsplit 38 and 37; 4096 x 128 x 4096 in 64 x 64 and 4
+// splits 19 and 21; 4096 x 70 x 14336 in 128 x 128 and 8 splits 29 and 30, in
+// 64 x 64 and 4 splits 41 and 36.
 struct TilePlan {
     int kind, splits;
 };
@@ -700,7 +702,7 @@ static TilePlan tile_plan(int64_t M, int64_t N, int steps, size_t ws_bytes) {
     static const struct {
         int bm, bn;
         double base, more;
-    } kinds[] = {{224, 256, 0, 3.4}, {128, 256, 0, 2.2}, {128, 128, 0.3, 1.1}, {64, 64, 0.35, 0.34}};
+    } kinds[] = {{224, 256, 0, 3.4}, {128, 256, 0, 2.2}, {128, 128, 0.3, 1.1}, {64, 64, 0.35, 0.42}};
     TilePlan best{2, 1};
     double least = 0;
     for (int k = 0; k < 4; ++k)
@@ -710,7 +712,7 @@ static TilePlan tile_plan(int64_t M, int64_t N, int steps, size_t ws_bytes) {
             const int64_t tiles = ((M + kinds[k].bm - 1) / kinds[k].bm) * ((N + kinds[k].bn - 1) / kinds[k].bn);
             const double c = (double) ((tiles * splits + 255) / 256);
             const double t = (steps + splits - 1) / splits * (kinds[k].base + c * kinds[k].more) +
-                             (splits > 1 ? 3 + 2 * planes / 5e6 : 0);
+                             (splits > 1 ? 5 + 2 * planes / 4e6 : 0);
             if (least == 0 || t < least) {
                 least = t;
                 best = {k, splits};
@@ -771,7 +773,7 @@ static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipSt
     } else if (plan.kind == 1) {
         launch_tile<4, 4, 2, 4>(p, splits, s);
     } else if (plan.kind == 2) {
-        launch_tile<4, 2, 2, 4>(p, splits, s);
+        launch_tile<2, 4, 4, 2>(p, splits, s);
     } else {
         launch_tile<2, 2, 2, 2>(p, splits, s);
     }
