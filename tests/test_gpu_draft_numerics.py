@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import draft_ref as ref
-from test_gpu_draft import HALF, TREES, bf, val
+from test_gpu_draft import HALF, TREES, bf, head_norm_case, val
 from test_gpu_mxfp4 import Graph
 
 pytestmark = pytest.mark.gpu
@@ -105,6 +105,16 @@ def test_rising_and_falling_scores(wx, be, rng, t, heads, kv, dh, past, step):
     slots = np.arange(k.shape[2]) % 2000
     k[..., 0] = wx.f32_to_bf16((slots * step).astype(np.float32))
     close(wx, run(wx, be, q, k, v, par, past, 1.0), q, k, v, par, past, 1.0)
+
+
+@pytest.mark.parametrize("t", [1, 8, 64, 130])
+def test_appends_at_every_place_in_a_tile(wx, be, rng, t):
+    """V^T is written eight slots at a time where all eight are new; the slots
+    beside them keep what they hold."""
+    print(f"append t {t}", flush=True)
+    past = [0, 1, 7, 8, 57, 63, 64, 65, 200 - t]
+    head_norm_case(wx, be, rng, len(past), t, 2, 1, 64, 64, 2, past, 200)
+    head_norm_case(wx, be, rng, len(past), t, 2, 2, 128, 32, 0, past, 203, ld_pad=5)
 
 
 def test_two_split_graphs_replayed_between_single_calls(wx, be):

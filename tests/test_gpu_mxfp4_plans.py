@@ -17,6 +17,7 @@ pytestmark = pytest.mark.gpu
 TILES = [(6963, 1175, 256), (4350, 1172, 5024), (1753, 1183, 4960), (4289, 1162, 256), (1056, 1159, 3904),
          (2745, 1140, 256), (1601, 938, 3040), (837, 845, 3008), (515, 661, 4032), (75, 68, 256), (70, 66, 1280),
          (65, 71, 2112), (69, 66, 4096), (7000, 2049, 64), (6500, 50, 96)]
+TILES += [(1829, 1106, 5024), (974, 1039, 3360), (2707, 130, 4800), (590, 769, 2848), (65, 72, 1760)]
 # One to four tiles of tokens by one, two and four groups of rows, and four K splits.
 FEW = [(40, 9, 96), (40, 30, 96), (40, 47, 96), (40, 64, 96), (6405, 9, 64), (6405, 30, 64), (6390, 41, 64), (6390, 64, 64),
        (12805, 16, 64), (12805, 17, 64), (12805, 33, 64), (1000, 35, 12288), (1030, 64, 12320), (2060, 40, 12288),

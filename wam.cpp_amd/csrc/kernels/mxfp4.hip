@@ -172,10 +172,13 @@ __global__ __launch_bounds__(kQThreads) void mx_quantize(const T * __restrict__ 
     }
 }
 
-// Values of packed blocks: the reverse path (blocks through LDS, eight values
-// per lane).  ldy is the row stride of y in elements; qs the byte stride of
-// packed rows (row_blocks * 17 when they follow each other); rows (nullable)
-// picks row rows[r] of `qrows` packed rows (negative or past the end: NaN).
+// Values of packed blocks: the reverse path, four lanes to a block, eight codes
+// read and eight values written by each.  ldy is the row stride of y in
+// elements; qs the byte stride of packed rows (row_blocks * 17 when they follow
+// each other); rows (nullable) picks row rows[r] of `qrows` packed rows
+// (negative or past the end: NaN).  Bound by its writes: 14336 x 4096 values to
+// f32 44 us, 6.1 TB/s over reads and writes that the caches still hold; with
+// the quantisation that precedes it 116 us, 4.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kQThreads) void mx_dequantize(const uint8_t * __restrict__ q, int64_t qs,
                                                            const int32_t * __restrict__ rows, int64_t qrows,
