@@ -628,7 +628,7 @@ WAMX_API wamx_status wamx_op_quantize_mxfp4(wamx_backend_t be, const void * x, i
 WAMX_API wamx_status wamx_op_dequantize_mxfp4(wamx_backend_t be, const void * q, void * y, int32_t y_type, int64_t ldy,
                                               int64_t rows, int64_t cols);
 /* wamx_op_mul_mat and wamx_op_linear with w in MXFP4 rows [M][K], K a multiple
- * of 32: x (bf16, or f32 rounded to bf16), f32 accumulation, any N. */
+ * of 32 below 2^30: x (bf16, or f32 rounded to bf16), f32 accumulation, any N. */
 WAMX_API wamx_status wamx_op_mul_mat_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type, int64_t ldx,
                                            void * y, int32_t y_type, int64_t ldy, int64_t M, int64_t N, int64_t K);
 WAMX_API wamx_status wamx_op_linear_mxfp4(wamx_backend_t be, const void * w, const void * x, int32_t x_type,

@@ -8,7 +8,7 @@ import pytest
 
 import draft_ref as ref
 from test_gpu_draft import HALF, TREES, bf, head_norm_case, val
-from test_gpu_mxfp4 import Graph
+from test_gpu_mxfp4 import Graph, int_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,39 @@ def test_two_split_graphs_replayed_between_single_calls(wx, be):
             np.testing.assert_array_equal(got, run(wx, be, q, k, v, par, now))
     for g, *_ in graphs:
         g.close()
+
+
+def test_split_kernels_on_two_lanes(wx, be):
+    """A split 4-bit product on one lane beside a split attention on the other,
+    each with a workspace of its lane; the attention's result meets the product's
+    next weight.  Replayed, and equal to the single calls."""
+    lib, rng = be.lib, np.random.default_rng(6)
+    M, N, K, t, heads, kv, dh = 256, 40, 12288, 5, 4, 2, 64
+    q, k, v, par, past = inputs(wx, rng, t, heads, kv, dh, [2900, 700])
+    cap = v.shape[3]
+    k = np.concatenate([k, k[:, :, :cap - k.shape[2]]], 2)
+    g, B, BF, I = Graph(wx, be), 2, wx.TYPE_BF16, wx.TYPE_I32
+    w, x, w2 = g.leaf(wx.TYPE_MXFP4, K, M), g.leaf(BF, K, N), g.leaf(wx.TYPE_MXFP4, heads * dh, 96)
+    tq, tk, tv = g.leaf(BF, dh, t, heads, B), g.leaf(BF, dh, cap, kv, B), g.leaf(BF, cap, dh, kv, B)
+    tpar, tpast = g.leaf(I, t, B), g.leaf(I, B)
+    g.place()
+    lib.wamx_set_lane(g.ctx, 1)
+    at = lib.wamx_tree_attn(g.ctx, tq, tk, tv, tpar, tpast, dh ** -0.5)
+    y2 = lib.wamx_mul_mat(g.ctx, w2, lib.wamx_reshape_2d(g.ctx, at, heads * dh, B * t))
+    lib.wamx_set_lane(g.ctx, 0)
+    y = lib.wamx_mul_mat(g.ctx, w, x)
+    g.build(y, y2)
+    w2v = ref.quantize(rng.standard_normal((96, heads * dh)) * 0.05)
+    for leaf, a in ((tq, q), (tk, k), (tv, v), (tpar, par), (w2, w2v)):
+        g.set(leaf, a)
+    for step in range(4):
+        wv, xv = int_weights(rng, M, K), rng.integers(-3, 4, (N, K)).astype(np.float32)
+        now = (past - 500 * (step % 2)).astype(np.int32)
+        g.set(w, wv), g.set(x, wx.f32_to_bf16(xv)), g.set(tpast, now)
+        g.compute()
+        np.testing.assert_array_equal(g.get(y, np.float32, (N, M)), xv @ ref.dequantize(wv).astype(np.float32).T)
+        a = wx.f32_to_bf16(run(wx, be, q, k, v, par, now).reshape(B * t, heads * dh).astype(np.float32))
+        d, dw, out = be.array(a), be.array(w2v), be.empty(B * t * 96 * 4)
+        wx.check(lib.wamx_op_mul_mat_mxfp4(be.ptr, dw.ptr, d.ptr, BF, heads * dh, out.ptr, wx.TYPE_F32, 96, 96, B * t, heads * dh))
+        np.testing.assert_array_equal(g.get(y2, np.float32, (B * t, 96)), out.download(np.float32, (B * t, 96)))
+    g.close()

@@ -1090,7 +1090,7 @@ static bool supports(const wamx_tensor * t) {
                 return false;
             if (tensor_is_tiled(s0)) return tiled_product_ok(s1) && wamx_is_contiguous(t);
             if (is_mxfp4(s0))
-                return s0->ne[0] > 0 && s0->ne[0] % wamx_blck_size(s0->type) == 0 && rows_contig(s0) &&
+                return s0->ne[0] > 0 && s0->ne[0] < 1 << 30 && s0->ne[0] % wamx_blck_size(s0->type) == 0 && rows_contig(s0) &&
                        (s1->type == WAMX_TYPE_BF16 || s1->type == WAMX_TYPE_F32) && rows_contig(s1) &&
                        s1->nb[1] % es(s1) == 0 && s1->nb[2] % es(s1) == 0 && s1->nb[3] % es(s1) == 0 &&
                        wamx_is_contiguous(t);
@@ -2154,8 +2154,8 @@ wamx_status wamx_op_mul_mat_mxfp4(wamx_backend_t be, const void * w, const void 
     WAMX_REQUIRE(be && w && x && y, "wamx_op_mul_mat_mxfp4: null argument");
     WAMX_REQUIRE(x_type == WAMX_TYPE_F32 || x_type == WAMX_TYPE_BF16, "wamx_op_mul_mat_mxfp4: x type");
     WAMX_REQUIRE(y_type == WAMX_TYPE_F32 || y_type == WAMX_TYPE_BF16, "wamx_op_mul_mat_mxfp4: y type");
-    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0 && ldx >= K && ldy >= M,
-                 "wamx_op_mul_mat_mxfp4: sizes (K a multiple of 32)");
+    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0 && K < 1 << 30 && ldx >= K && ldy >= M,
+                 "wamx_op_mul_mat_mxfp4: sizes (K a multiple of 32 below 2^30)");
     MxArgs a;
     a.w = w;
     a.w_stride = mx_row_bytes(K);
@@ -2179,7 +2179,8 @@ wamx_status wamx_op_linear_mxfp4(wamx_backend_t be, const void * w, const void *
                                  int64_t N, int64_t K) {
     WAMX_REQUIRE(be && w && x && y, "wamx_op_linear_mxfp4: null argument");
     WAMX_REQUIRE(x_type == WAMX_TYPE_F32 || x_type == WAMX_TYPE_BF16, "wamx_op_linear_mxfp4: x type");
-    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0, "wamx_op_linear_mxfp4: sizes (K a multiple of 32)");
+    WAMX_REQUIRE(M >= 0 && N >= 0 && K > 0 && K % 32 == 0 && K < 1 << 30,
+                 "wamx_op_linear_mxfp4: sizes (K a multiple of 32 below 2^30)");
     WAMX_REQUIRE(epilogue >= WAMX_EPI_NONE && epilogue <= WAMX_EPI_BIAS_RESIDUAL, "wamx_op_linear_mxfp4: epilogue");
     WAMX_REQUIRE(epilogue == WAMX_EPI_NONE || bias, "wamx_op_linear_mxfp4: bias required");
     WAMX_REQUIRE((epilogue != WAMX_EPI_BIAS_GATED && epilogue != WAMX_EPI_BIAS_RESIDUAL) || residual,

@@ -122,7 +122,7 @@ const char * check_linear(const wamx_tensor * t) {
     if ((!is_bf16(w) && !mx) || !x || (x->type != WAMX_TYPE_BF16 && x->type != WAMX_TYPE_F32)) return "types";
     if (w->ne[0] != x->ne[0] || w->ne[2] != 1 || w->ne[3] != 1 || x->ne[2] != 1 || x->ne[3] != 1) return "shapes";
     if (w->nb[0] != wamx_type_size(w->type) || x->nb[0] != wamx_type_size(x->type)) return "rows must be contiguous";
-    if (mx && w->ne[0] % wamx_blck_size(w->type) != 0) return "rows of whole blocks";
+    if (mx && (w->ne[0] % wamx_blck_size(w->type) != 0 || w->ne[0] >= 1 << 30)) return "rows of whole blocks, below 2^30";
     const int64_t M = w->ne[1], N = x->ne[1];
     if (epi < WAMX_EPI_NONE || epi > WAMX_EPI_BIAS_RESIDUAL) return "epilogue";
     if (epi != WAMX_EPI_NONE && (!is_bf16(bias) || bias->ne[0] != M || bias->nb[0] != 2)) return "bias";
