@@ -76,6 +76,30 @@ __device__ __forceinline__ void tree_paths(TreePaths & path, void * work, int pa
     }
 }
 
+// The same for at most 64 tokens, lane i's in a register of every wave.
+__device__ __forceinline__ uint64_t tree_path(int parent, int tq) {
+    const int lane = threadIdx.x & 63;
+    int jump = parent >= 0 && parent < tq ? parent : -1;
+    const bool token = lane < tq && parent >= -1 && parent < tq;
+    uint32_t lo = token && lane < 32 ? 1u << lane : 0u, hi = token && lane >= 32 ? 1u << (lane - 32) : 0u;
+    for (int reach = 1; reach < tq; reach *= 2) {
+        const int from = max(jump, 0), next = __shfl(jump, from);
+        const uint32_t l = (uint32_t) __shfl((int) lo, from), h = (uint32_t) __shfl((int) hi, from);
+        if (jump >= 0) {
+            lo |= l;
+            hi |= h;
+            jump = next;
+        }
+    }
+    return (uint64_t) hi << 32 | lo;
+}
+// Four bits of it from drafted slot `off` on (negative: still in the cache).
+__device__ __forceinline__ uint32_t tree_seen4(uint64_t path, int64_t off) {
+    if (off >= 64) return 0u;
+    if (off >= 0) return (uint32_t) (path >> off);
+    return off <= -4 ? 15u : (uint32_t) path << -off | ((1u << -off) - 1);
+}
+
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
 // The offset that a row's exponents are taken from: its first maximum, raised
@@ -214,8 +238,6 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     __shared__ __align__(16) uint16_t qs[R * DH];
     __shared__ __align__(16) uint16_t ps[R * TILE];
     __shared__ float sm[kTreeWaves][R];
-    __shared__ TreePaths path;
-    __shared__ TreeWork work;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
@@ -234,7 +256,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     tree_range(n, u - unit.first, unit.count, t0, t1);
     const int64_t bz = (int64_t) b * p.kv_heads + hk;
     const int32_t * parents = p.parents + (int64_t) b * p.tq;
-    const int parent = (int) threadIdx.x < p.tq ? parents[threadIdx.x] : -1;
+    const int parent = lane < p.tq ? parents[lane] : -1;
 
     const uint16_t * kb = p.k + bz * p.capacity * DH + g * 8;
     const uint16_t * vb = p.vt + (bz * DH + wave * (DH / 4) + c16) * p.vt_ld;
@@ -273,7 +295,13 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
         const int pr = parents[tok[i]];
         token[i] = pr >= -1 && pr < p.tq;
     }
-    if (t0 < t1 && t1 * TILE > past) tree_paths(path, &work, parent, p.tq);
+    uint64_t path[NR] = {};
+    if (t0 < t1 && t1 * TILE > past) {
+        const uint64_t mine = tree_path(parent, p.tq);
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            path[i] = (uint64_t) (uint32_t) __shfl((int) (mine >> 32), tok[i]) << 32 | (uint32_t) __shfl((int) mine, tok[i]);
+    }
     __syncthreads();
 
     float m[NR], l[NR];
@@ -304,7 +332,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             if (edge) {
-                const uint32_t seen = tree_seen(path[tok[i]], base + wave * 16 + 4 * g - past, p.tq);
+                const uint32_t seen = tree_seen4(path[i], base + wave * 16 + 4 * g - past);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[i][r] = seen >> r & 1 ? s[i][r] : -INFINITY;
             }
@@ -370,7 +398,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
             const int a = (int) (slot - past);
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                if (!(path[tok[i]][a >> 5] >> (a & 31) & 1)) continue;
+                if (!(path[i] >> a & 1)) continue;
                 const int row = min(row0 + i * 16 + c16, rows - 1);
                 const float pr =
                     tree_weight(p, b, hk * group + row / p.tq, tok[i], kb - g * 8 + slot * DH, DH, m[i]);
