@@ -338,7 +338,7 @@ static hipError_t run_mxfp4_copy(wamx_backend * be, const wamx_tensor * src, con
     return hipSuccess;
 }
 
-static hipError_t run_head_norm_rope(wamx_backend * be, const wamx_tensor * node) {
+static HeadNormArgs head_norm_args(const wamx_tensor * node) {
     const wamx_tensor *x = node->src[0], *dst = node->src[2];
     const bool vt = node->op_params[4] != 0;
     HeadNormArgs a;
@@ -362,7 +362,7 @@ static hipError_t run_head_norm_rope(wamx_backend * be, const wamx_tensor * node
         memcpy(&a.freq_base, &node->op_params[3], 4);
         a.pos = a.n_dims > 0 ? (const int32_t *) node->src[4]->data : nullptr;
     }
-    return launch_head_norm_rope(a, be->cs);
+    return a;
 }
 
 static hipError_t run_tree_attn(wamx_backend * be, const wamx_tensor * node) {
@@ -437,6 +437,7 @@ static float param_f32(const wamx_tensor * t, int i) {
 //   * LINEAR -> NORM of its output (LayerNorm / adaLN modulation), the
 //     residual-stream pattern h = lin(..., h); n = norm(h) of mot.cpp:130-145,
 //     284-346;
+//   * HEAD_NORM_ROPE of queries, keys and values -> one launch;
 //   * LINEAR -> up to three of QK_NORM_ROPE of a column range and the V^T
 //     copy (CPY of a permuted column range), the QKV split of mot.cpp:245-265,
 //     395-401.
@@ -465,6 +466,90 @@ static int next_compute(wamx_cgraph * g, int i, int n, bool lanes) {
         if (!is_noop(t) && (!lanes || t->lane == lane)) return j;
     }
     return n;
+}
+
+static bool memory_meets(const wamx_tensor * a, const wamx_tensor * b) {
+    return a && b && (const char *) a->data < (const char *) b->data + wamx_nbytes(b) &&
+           (const char *) b->data < (const char *) a->data + wamx_nbytes(a);
+}
+
+// HEAD_NORM_ROPE nodes after one another, from node i on, that one launch
+// computes: a step's queries (a destination of T rows, no lengths), keys and
+// V^T append, in any order, from rows of one stride.  A node that reads or writes
+// what another of them writes ends the group.  Their number, with the launch's
+// arguments and the nodes' indices.  (One token of 24 + 24 + 24 heads of 128 in a
+// replayed graph: 4.5 us, node by node 9.6.)
+static int match_head_norms(wamx_cgraph * g, int i, int n, bool lanes, HeadNormArgs & a, int * members) {
+    const wamx_tensor * nodes[3];
+    HeadNormArgs parts[3];
+    int role[3], count = 0;  // 0 queries, 1 keys, 2 values
+    bool taken[3] = {false, false, false};
+    for (int j = i; j < n && count < 3; j = next_compute(g, j, n, lanes)) {
+        const wamx_tensor * t = wamx_graph_node(g, j);
+        if (t->op != WAMX_OP_HEAD_NORM_ROPE) break;
+        bool data = t->data != nullptr;
+        for (int k = 0; k < 5; ++k) data = data && (!t->src[k] || t->src[k]->data);
+        if (!data || check_head_norm_rope(t)) break;
+        const HeadNormArgs p = head_norm_args(t);
+        const int r = p.vt ? 2 : !taken[0] && !p.past && p.k_rows == p.tokens ? 0 : 1;
+        bool fits = !taken[r];
+        for (int m = 0; m < count && fits; ++m) {
+            const HeadNormArgs & o = parts[m];
+            fits = p.ldx == o.ldx && p.batch == o.batch && p.tokens == o.tokens && p.head_dim == o.head_dim;
+            if (r < 2 && role[m] < 2)
+                fits = fits && p.rope_mode == o.rope_mode && p.n_dims == o.n_dims && p.eps == o.eps &&
+                       p.freq_base == o.freq_base && p.pos == o.pos;
+            if (r > 0 && role[m] > 0)
+                fits = fits && p.kv_heads == o.kv_heads && p.k_rows == o.k_rows && p.past == o.past;
+            for (int k = 0; k < 5; ++k)
+                fits = fits && !memory_meets(t->src[k], nodes[m]->src[2]) && !memory_meets(nodes[m]->src[k], t->src[2]);
+        }
+        if (!fits) break;
+        taken[r] = true;
+        nodes[count] = t;
+        parts[count] = p;
+        role[count] = r;
+        members[count++] = j;
+    }
+    if (count < 2) return count;
+    const uint16_t * first = (const uint16_t *) parts[0].x;
+    for (int m = 1; m < count; ++m) first = std::min(first, (const uint16_t *) parts[m].x);
+    a = parts[0];
+    a.x = first;
+    a.wk = a.k = a.vt = nullptr;
+    a.kv_heads = 0;
+    for (int m = 0; m < count; ++m) {
+        const HeadNormArgs & p = parts[m];
+        const int64_t col = (const uint16_t *) p.x - first;
+        if (((uintptr_t) p.x - (uintptr_t) first) % 2 != 0 || col > 0x7fffffff) return 1;
+        if (role[m] < 2) {
+            a.rope_mode = p.rope_mode;
+            a.n_dims = p.n_dims;
+            a.eps = p.eps;
+            a.freq_base = p.freq_base;
+            a.pos = p.pos;
+        }
+        if (role[m] == 0) {
+            a.wq = p.wk;
+            a.q = p.k;
+            a.heads = p.kv_heads;
+            a.q_col = col;
+            continue;
+        }
+        a.kv_heads = p.kv_heads;
+        a.k_rows = p.k_rows;
+        a.past = p.past;
+        if (role[m] == 1) {
+            a.wk = p.wk;
+            a.k = p.k;
+            a.k_col = col;
+        } else {
+            a.vt = p.vt;
+            a.vt_ld = p.vt_ld;
+            a.v_col = col;
+        }
+    }
+    return count;
 }
 
 // Column offset of x inside the rows of `base` (x is base, or a view taking a
@@ -960,7 +1045,7 @@ static hipError_t compute_node(wamx_backend * be, wamx_tensor * node) {
             return launch_euler_step(s0->data, s1->data, (const float *) node->src[2]->data, node->data,
                                      wamx_nelements(node), s);
         case WAMX_OP_HEAD_NORM_ROPE:
-            return run_head_norm_rope(be, node);
+            return launch_head_norm_rope(head_norm_args(node), s);
         case WAMX_OP_TREE_ATTN:
             return run_tree_attn(be, node);
         case WAMX_OP_MLP_SMALL:
@@ -1359,6 +1444,27 @@ static wamx_status run_nodes(wamx_backend * be, wamx_cgraph * g) {
             }
             if (!fused) {
                 nm = 1;
+                members[0] = i;
+            }
+        }
+        if (node->op == WAMX_OP_HEAD_NORM_ROPE && be->fuse_rows) {
+            HeadNormArgs a;
+            int dep = -1;
+            const int count = match_head_norms(g, i, n, two, a, members);
+            for (int m = 0; m < count; ++m) dep = std::max(dep, two ? wait_for[members[m]] : -1);
+            if (count > 1 && dep <= i) {
+                if (dep >= 0) hipStreamWaitEvent(be->cs, be->events[slot[dep]], 0);
+                const hipError_t err = launch_head_norm_rope(a, be->cs);
+                if (err != hipSuccess) {
+                    set_errorf("graph_compute: node %d (%s '%s') with the nodes after it failed: %s", i,
+                               wamx_op_name(node->op), node->name, hipGetErrorString(err));
+                    status = WAMX_STATUS_FAILED;
+                    break;
+                }
+                fused = true;
+                nm = count;
+                for (int m = 0; m < nm; ++m) done[members[m]] = 1;
+            } else {
                 members[0] = i;
             }
         }
