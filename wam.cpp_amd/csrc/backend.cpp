@@ -437,7 +437,6 @@ static float param_f32(const wamx_tensor * t, int i) {
 //   * LINEAR -> NORM of its output (LayerNorm / adaLN modulation), the
 //     residual-stream pattern h = lin(..., h); n = norm(h) of mot.cpp:130-145,
 //     284-346;
-//   * HEAD_NORM_ROPE of queries, keys and values -> one launch;
 //   * LINEAR -> up to three of QK_NORM_ROPE of a column range and the V^T
 //     copy (CPY of a permuted column range), the QKV split of mot.cpp:245-265,
 //     395-401.
