@@ -296,6 +296,20 @@ __device__ __forceinline__ bf16x8_t mx_frag(uint32_t d, float scale) {
     return u.v;
 }
 
+// The codes of a block with value j in nibble j: dword g holds 8g .. 8g + 7.
+__device__ __forceinline__ uint4 mx_natural(const any16 & b) {
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // Four nibbles to bytes 0 and 2.
+        const uint32_t l = b.v[i] & 0x0f0f0f0fu, h = (b.v[i] >> 4) & 0x0f0f0f0fu;
+        lo[i] = l | l >> 4;
+        hi[i] = h | h >> 4;
+    }
+    return make_uint4(__builtin_amdgcn_perm(lo[1], lo[0], 0x06040200u), __builtin_amdgcn_perm(lo[3], lo[2], 0x06040200u),
+                      __builtin_amdgcn_perm(hi[1], hi[0], 0x06040200u), __builtin_amdgcn_perm(hi[3], hi[2], 0x06040200u));
+}
+
 // The activations of mx_frag(dword i): values 4i .. 4i + 3 (lo) and 16 + 4i ..
 // (hi) of the block, paired in the same order.
 __device__ __forceinline__ bf16x8_t mx_pair(uint32_t lo0, uint32_t lo1, uint32_t hi0, uint32_t hi1) {
@@ -472,20 +486,22 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
 // Many tokens: WM waves along the weight rows by WN along the tokens, each RG x
 // NT tiles of 16 x 16.  Every wave expands its rows' codes itself, so 128 x 128
 // tiles take 4 x 2 waves of 2 x 4 tiles (10250 x 333 x 2048: 28.9 us, 2 x 4
-// waves of 4 x 2 tiles 30.5).  The weight stays in its 4 bits down to the register
-// that becomes the operand: a step of 128 values is 4 blocks a row, whose codes
-// lie in LDS as [block][row][g], so that a wave's read of dword g of its rows is
-// 256 bytes in a row.  Such a dword
-// expands to values (4g + t, 16 + 4g + t), t = 0..3, of its block, and x is
-// written to LDS in that order (two 16-byte pieces 16 values apart, interleaved
-// on the way), half a step at a time.  Both go through registers, requested a
-// step before their use, into one of two LDS buffers while the other is
-// multiplied: one barrier per half step, the writes behind the first row tile's
-// products.
+// waves of 4 x 2 tiles 30.5).  The weight stays in its 4 bits down to the
+// register that becomes the operand: a step of 128 values is 4 blocks a row,
+// whose codes are put into the order of their values on the way to LDS and lie
+// there as [block][row][g], so that a wave's read of dword g of its rows is 256
+// bytes in a row and expands to values 8g .. 8g + 7 of its block.  x lies in LDS
+// as it is, half a step at a time.  (With x interleaved in the codes' own order
+// instead, and the blocks read at odd addresses for want of registers: 4096 x
+// 1100 x 4096 67.7 us for 63.5, 14336 x 2048 x 4096 215 for 210, 10250 x 333 x
+// 2048 28.9 for 27.7.)  Both go through registers, requested a step before their
+// use, into one of two LDS buffers while the other is multiplied: one barrier
+// per half step, the writes behind the first row tile's products.  x straight
+// into LDS, three buffers, took as long or longer: 221 us for 2048 tokens.
 template <int RG, int NT, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
     constexpr int TH = 64 * WM * WN, BM = RG * 16 * WM, BN = NT * 16 * WN;
-    constexpr int XP = BN * 4 / TH;             // pairs of x pieces of a thread per half step
+    constexpr int XP = BN * 8 / TH;             // 16-byte x pieces of a thread per half step
     constexpr int WB = (BM * 4 + TH - 1) / TH;  // weight blocks of a thread per step
     // The four blocks of a row, written by four neighbouring lanes, lie a
     // quarter of the banks apart.
@@ -506,28 +522,31 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
     // Weight blocks: thread t takes block t % 4 of rows t / 4, t / 4 + TH / 4, ...
     const int wkb = threadIdx.x & 3, wrow = threadIdx.x >> 2;
     uint32_t woff[WB];
+    const uint32_t wlow = (uint32_t) (uintptr_t) wbase;
 #pragma unroll
     for (int j = 0; j < WB; ++j)
         woff[j] = (uint32_t) min((int64_t) (wrow + j * (TH / 4)), p.M - 1 - m0) * (uint32_t) p.ws;
-    // (Loads at odd addresses: the five dwords of mx_load cost registers that
-    // the large tiles do not have, 14336 x 2048 x 4096 in 224 us against 210.)
-    any16 wr[WB];
-    uint32_t wsc[WB];
-    auto request_w = [&](int s, any16 * r, uint32_t * e) {
+    MxBlock wr[WB];
+    uint32_t wmis[WB];
+    auto request_w = [&](int s, MxBlock * r, uint32_t * e) {
         const uint32_t at = (uint32_t) min(4 * s + wkb, p.kb - 1) * (uint32_t) kMxBytes;
 #pragma unroll
         for (int j = 0; j < WB; ++j) {
-            r[j] = *(const any16 *) (wbase + (woff[j] + at + 1u));
-            e[j] = *(const uint8_t *) (wbase + (woff[j] + at));
+            const uint32_t o = woff[j] + at;
+            e[j] = (wlow + o) & 3;
+            r[j] = mx_load(wbase + (int64_t) o - e[j]);
         }
     };
-    auto deposit_w = [&](int s, int buf, const any16 * r, const uint32_t * e) {
+    auto deposit_w = [&](int s, int buf, const MxBlock * r, const uint32_t * e) {
 #pragma unroll
         for (int j = 0; j < WB; ++j) {
             const int row = wrow + j * (TH / 4);
             if (BM % (TH / 4) != 0 && row >= BM) break;
-            ((uint4 *) wl[buf])[wkb * WS + row] = make_uint4(r[j].v[0], r[j].v[1], r[j].v[2], r[j].v[3]);
-            sl[buf][wkb * SS + row] = mx_scale(e[j]);
+            any16 c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c.v[i] = mx_codes(r[j], i, mx_select(e[j]));
+            ((uint4 *) wl[buf])[wkb * WS + row] = mx_natural(c);
+            sl[buf][wkb * SS + row] = mx_scale(mx_exponent(r[j], e[j]));
         }
         if (4 * s + 4 > p.kb && 4 * s + wkb >= p.kb) {  // past a row's last block: zeros
 #pragma unroll
@@ -539,36 +558,29 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
             }
         }
     };
-    // Activations: a pair is the pieces at 8c and 16 + 8c (c = 0, 1) of block
-    // xi = 0, 1 of a half step.
-    const int xi = (threadIdx.x >> 1) & 1, xc = threadIdx.x & 1;
-    any16 xr[2][XP][2];
+    // Activations: eight lanes read the 128 bytes of a row's half step.
+    const int xc = threadIdx.x & 7;
+    any16 xr[2][XP];
     uint32_t xoff[XP];
     int xpos[XP];
 #pragma unroll
     for (int q = 0; q < XP; ++q) {
-        const int row = (threadIdx.x >> 2) + q * (TH / 4);
-        xoff[q] = ((uint32_t) min((int64_t) row, p.N - 1 - n0) * (uint32_t) p.ldx + (uint32_t) xc * 8) * 2;
-        xpos[q] = row * 8 + ((xi * 4 + xc * 2) ^ ((row >> 1) & 7));  // slot of operand g = 2c; g + 1 in slot ^ 1
+        const int row = (threadIdx.x >> 3) + q * (TH / 8);
+        xoff[q] = ((uint32_t) min((int64_t) row, p.N - 1 - n0) * (uint32_t) p.ldx + (uint32_t) (xc & 3) * 8) * 2;
+        xpos[q] = row * 8 + (xc ^ ((row >> 1) & 7));
     }
-    auto request_x = [&](int h, any16 (*r)[2]) {  // half step h: blocks 2h, 2h + 1
-        const uint32_t at = (uint32_t) min(2 * h + xi, p.kb - 1) * 64u;
+    auto request_x = [&](int h, any16 * r) {  // half step h: blocks 2h, 2h + 1
+        const uint32_t at = (uint32_t) min(2 * h + (xc >> 2), p.kb - 1) * 64u;
 #pragma unroll
-        for (int q = 0; q < XP; ++q) {
-            r[q][0] = *(const any16 *) (xbase + (xoff[q] + at));
-            r[q][1] = *(const any16 *) (xbase + (xoff[q] + at + 32u));
-        }
+        for (int q = 0; q < XP; ++q) r[q] = *(const any16 *) (xbase + (xoff[q] + at));
     };
-    auto deposit_x = [&](int h, int buf, any16 (*r)[2]) {
-        bf16x8_t * dst = (bf16x8_t *) xl[buf];
+    auto deposit_x = [&](int h, int buf, const any16 * r) {
+        uint4 * dst = (uint4 *) xl[buf];
 #pragma unroll
-        for (int q = 0; q < XP; ++q) {
-            dst[xpos[q]] = mx_pair(r[q][0].v[0], r[q][0].v[1], r[q][1].v[0], r[q][1].v[1]);
-            dst[xpos[q] ^ 1] = mx_pair(r[q][0].v[2], r[q][0].v[3], r[q][1].v[2], r[q][1].v[3]);
-        }
-        if (2 * h + 2 > p.kb && 2 * h + xi >= p.kb) {
+        for (int q = 0; q < XP; ++q) dst[xpos[q]] = make_uint4(r[q].v[0], r[q].v[1], r[q].v[2], r[q].v[3]);
+        if (2 * h + 2 > p.kb && 2 * h + (xc >> 2) >= p.kb) {
 #pragma unroll
-            for (int q = 0; q < XP; ++q) dst[xpos[q]] = dst[xpos[q] ^ 1] = (bf16x8_t){};
+            for (int q = 0; q < XP; ++q) dst[xpos[q]] = make_uint4(0, 0, 0, 0);
         }
     };
 
@@ -601,12 +613,12 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
     // Requests past the last step repeat its addresses (requested, not used).
     const int last = s1 - 1;
     if (s0 < s1) {
-        request_w(s0, wr, wsc);
+        request_w(s0, wr, wmis);
         request_x(2 * s0, xr[0]);
         request_x(2 * s0 + 1, xr[1]);
-        deposit_w(s0, 0, wr, wsc);
+        deposit_w(s0, 0, wr, wmis);
         deposit_x(2 * s0, 0, xr[0]);
-        request_w(min(s0 + 1, last), wr, wsc);
+        request_w(min(s0 + 1, last), wr, wmis);
         request_x(2 * min(s0 + 1, last), xr[0]);
     }
     lds_barrier();
@@ -619,9 +631,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile(MxParams p) {
         lds_barrier();
         multiply(wb, 1, [&]() {
             deposit_x(2 * s + 2, 0, xr[0]);
-            deposit_w(s + 1, wb ^ 1, wr, wsc);
+            deposit_w(s + 1, wb ^ 1, wr, wmis);
             request_x(2 * min(s + 2, last), xr[0]);
-            request_w(min(s + 2, last), wr, wsc);
+            request_w(min(s + 2, last), wr, wmis);
         });
         lds_barrier();
     }
