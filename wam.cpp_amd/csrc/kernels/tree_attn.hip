@@ -697,7 +697,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
 
 // out = sum_s po_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over a row's units, DH / 4
 // threads with four values each.  BY_ROWS: 1024 / DH rows of one (sequence, key
-// head) to a workgroup, each thread over all units (many rows of few units);
+// head) to a workgroup, each thread over all units;
 // else one row, its units shared out among as many groups of threads, whose
 // results are added in order.
 template <int DH, bool BY_ROWS>
@@ -803,9 +803,10 @@ static hipError_t launch(void (*kernel)(TreeParams), int R, int threads, int64_t
     if (wgs > 0x7fffffff || joins > 0x7fffffff) return hipErrorInvalidValue;
     hipLaunchKernelGGL(kernel, dim3((unsigned) wgs), dim3((unsigned) threads), 0, s, p);
     if (p.po) {
-        // Many rows have few units each (64 tokens of 4 x 8 heads, 8 units: a
-        // workgroup per row 16.6 us), few rows many.
-        if (p.units <= 16 * a.batch) {
+        // Many rows fill the GPU by workgroups of rows (64 tokens of 4 x 32 heads
+        // 85 us in all, a workgroup per row 101; 4 tokens of 16 x 32 heads 21,
+        // 25), few by workgroups of one (33 tokens of 3 x 8: 34 us, by rows 35).
+        if (joins > 1024) {
             const int parts = (int) ((rows + 1024 / DH - 1) / (1024 / DH));
             hipLaunchKernelGGL((tree_attn_join<DH, true>), dim3((unsigned) (a.batch * a.kv_heads * parts)), dim3(256), 0, s,
                                p, parts);
