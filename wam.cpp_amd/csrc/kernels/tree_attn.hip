@@ -231,7 +231,9 @@ __device__ __forceinline__ void lds_barrier() {
 // dimensions for all rows and slots, so every K and V element is loaded once,
 // by one wave, into the registers that feed its matrix operand.  The rows (Q)
 // and the probabilities lie in LDS.  K of the next tile is requested when this
-// tile's scores are done and V when its product is.
+// tile's scores are done and V when its product is.  The slots' bytes bound it:
+// one token of 2 x 16 heads of 64 (4 key heads) over 100000 slots 37 to 39 us
+// with the join, 4.6 to 4.9 TB/s.
 template <int DH, int NR>
 __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 64, TILE = 64, R = NR * 16, QCH = DH / 8;
@@ -455,7 +457,13 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
 // interleaved (row a of tile u is slot 8 (a / 4) + 4 (u % 2) + a % 4 of its
 // half) eight consecutive slots in its registers: the operand of O^T = V^T P^T
 // as it stands.  K and V^T tiles of 64 slots go through registers into one of
-// two LDS buffers while the other is used; one barrier a tile.
+// two LDS buffers while the other is used; one barrier a tile.  A tile of 128
+// dimensions takes 5 k cycles for 2 k each of MFMA, exponentials with their sums
+// and LDS reads: 64 tokens of 4 x 32 heads (8 key heads) over 16000 slots 85 us
+// with the join, 0.64 PFLOP/s.  Two row tiles a wave in eight waves; four in four
+// waves of 512 registers 106 us, two in four 99.  What is not to be seen of V is
+// taken out once, on its way to LDS (100 tokens of 2 x 8 heads of 256 over 4000
+// slots 34 us, by every wave that reads it 43).
 template <int DH, int NR, int W>
 __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 16, TILE = 64, R = W * NR * 16, QCH = DH / 8;
@@ -463,6 +471,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
     __shared__ __align__(16) uint16_t kt_lds[2][TILE * DH];
     __shared__ __align__(16) uint16_t vt_lds[2][DH * TILE];
     __shared__ TreePaths path;
+    __shared__ int bad;  // Inf or NaN among the drafted values
     static_assert(sizeof(TreeWork) <= sizeof vt_lds, "the paths' scratch lies in the value tiles");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
             sr[j] = *(const bf16x8_t *) (kb + min(kt * TILE + e / QCH, n - 1) * DH + e % QCH * 8);
         }
     };
-    auto request_v = [&](int64_t kt) {
+    auto request_v = [&](int64_t kt, bf16x8_t * sr) {
 #pragma unroll
         for (int j = 0; j < VN; ++j) {
             const int e = threadIdx.x + j * W * 64;
@@ -515,14 +524,27 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
             *(bf16x8_t *) (kt_lds[buf] + k * DH + ((e % QCH) ^ kswz(k)) * 8) = sr[j];
         }
     };
-    auto deposit_v = [&](int buf) {
+    // A tile that reaches past the cache is looked over on its way.
+    auto deposit_v = [&](int64_t kt, int buf, const bf16x8_t * sr) {
+        const bool edge = (kt + 1) * TILE > past;
 #pragma unroll
         for (int j = 0; j < VN; ++j) {
             const int e = threadIdx.x + j * W * 64, d = e >> 3;
-            *(bf16x8_t *) (vt_lds[buf] + d * TILE + ((e & 7) ^ ((d >> 1) & 7)) * 8) = sr[j];
+            union {
+                bf16x8_t v;
+                uint32_t w[4];
+            } u;
+            u.v = sr[j];
+            if (edge && tree_mask_values(u.w, kt * TILE + (e & 7) * 8, past, n)) bad = 1;
+            *(bf16x8_t *) (vt_lds[buf] + d * TILE + ((e & 7) ^ ((d >> 1) & 7)) * 8) = u.v;
         }
     };
-    if (t0 < t1) request_k(t0);
+    bf16x8_t first_v[VN];
+    if (t0 < t1) {
+        request_k(t0);
+        request_v(t0, first_v);
+    }
+    if (threadIdx.x == 0) bad = 0;
     int tok[NR];
     bf16x8_t qf[NR][KC];
 #pragma unroll
@@ -533,11 +555,19 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
 #pragma unroll
         for (int c = 0; c < KC; ++c) qf[i][c] = tree_q(p, qr + c * 32 + g * 8);
     }
-    if (t0 < t1 && t1 * TILE > past) tree_paths(path, vt_lds, parent, p.tq);
+    if (t0 < t1 && t1 * TILE > past) {
+        if (p.tq > 64) {
+            tree_paths(path, vt_lds, parent, p.tq);
+        } else if (wave == 0) {
+            const uint64_t mine = tree_path(parent, p.tq);
+            path[lane][0] = (uint32_t) mine;
+            path[lane][1] = (uint32_t) (mine >> 32);
+        }
+    }
+    __syncthreads();
     if (t0 < t1) {
         deposit_k(0);
-        request_v(t0);
-        deposit_v(0);
+        deposit_v(t0, 0, first_v);
     }
     __syncthreads();
 
@@ -550,7 +580,6 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0, 0, 0, 0};
     }
-    bool bad = false;
     // EDGE: a tile that reaches past the cache, where every slot is looked at.
     auto tile = [&](int64_t kt, auto edge_tag) __attribute__((always_inline)) {
         constexpr bool edge = decltype(edge_tag)::value;
@@ -575,7 +604,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
         }
         if (kt + 1 < t1) {
             deposit_k(buf ^ 1);
-            request_v(kt + 1);
+            request_v(kt + 1, sr);
         }
         if (row0 < rows) {
             bf16x8_t pf[NR][2];
@@ -631,24 +660,19 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int dr = d * 16 + c16;
-                    union {
-                        bf16x8_t v;
-                        uint32_t w[4];
-                    } u;
-                    u.v = *(const bf16x8_t *) (vt_lds[buf] + dr * TILE + ((4 * h + g) ^ ((dr >> 1) & 7)) * 8);
-                    if (edge) bad |= tree_mask_values(u.w, base + h * 32 + g * 8, past, n);
+                    const bf16x8_t vf = *(const bf16x8_t *) (vt_lds[buf] + dr * TILE + ((4 * h + g) ^ ((dr >> 1) & 7)) * 8);
 #pragma unroll
                     for (int i = 0; i < NR; ++i)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, pf[i][h], o[i][d], 0, 0, 0);
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[i][h], o[i][d], 0, 0, 0);
                 }
         }
-        if (kt + 1 < t1) deposit_v(buf ^ 1);
+        if (kt + 1 < t1) deposit_v(kt + 1, buf ^ 1, sr);
         lds_barrier();
     };
     const int64_t inner = max(t0, min(t1, past / TILE));
     for (int64_t kt = t0; kt < inner; ++kt) tile(kt, std::false_type{});
     for (int64_t kt = inner; kt < t1; ++kt) tile(kt, std::true_type{});
-    if (__any(bad)) {
+    if (bad) {
         // Inf or NaN among the drafted values: added element by element to the
         // rows whose path holds the slot.
         for (int64_t slot = max(t0 * TILE, past); slot < min(t1 * TILE, n); ++slot) {
