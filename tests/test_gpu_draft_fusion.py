@@ -124,3 +124,17 @@ def test_replays_with_other_lengths(wx, be, rng):
             np.testing.assert_array_equal(got[n], want[n])
         s.data["k"], s.data["v"] = got["k"], got["v"]
     s.g.close()
+
+
+def test_a_cache_view_off_its_alignment_is_refused(wx, be, rng):
+    """What the single call refuses, the graph's constructor does too."""
+    lib = be.lib
+    g, BF, I = Graph(wx, be), wx.TYPE_BF16, wx.TYPE_I32
+    q, v, par, past = g.leaf(BF, DH, 1, 1, 1), g.leaf(BF, 8, DH, 1, 1), g.leaf(I, 1, 1), g.leaf(I, 1)
+    store = g.leaf(BF, DH * 8 + 8)
+    g.place()
+    for offset, ok in ((0, True), (2, False), (8, False), (16, True)):
+        k = lib.wamx_view_4d(g.ctx, store, DH, 8, 1, 1, DH * 2, DH * 16, DH * 16, offset)
+        o = lib.wamx_tree_attn(g.ctx, q, k, v, par, past, 1.0)
+        assert bool(o) == ok and (ok or "16-byte aligned" in wx.last_error())
+    g.close()

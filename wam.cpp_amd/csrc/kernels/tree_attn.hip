@@ -856,6 +856,9 @@ static hipError_t run_many(TreeParams & p, const TreeArgs & a, hipStream_t s) {
 
 hipError_t launch_tree_attn(const TreeArgs & a, hipStream_t s) {
     if (a.tq <= 0 || a.batch <= 0) return hipSuccess;
+    // Wide reads of q, k and V^T, and result stores of two values.
+    if (((uintptr_t) a.q | (uintptr_t) a.k | (uintptr_t) a.vt) % 16 != 0 || (uintptr_t) a.out % 4 != 0)
+        return hipErrorInvalidValue;
     if (a.tq > kTreeMax || a.batch > 0x7fffffff / std::max<int64_t>(a.kv_heads, 1) || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.vt_ld % 8 != 0 ||
         a.vt_ld < a.capacity || a.capacity <= 0 || a.capacity > 0x7fffffff)
         return hipErrorInvalidValue;
