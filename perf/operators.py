@@ -136,20 +136,14 @@ def _dequantize(packed, dtype=torch.float32):
 # Inputs
 # ---------------------------------------------------------------------------
 _BE = None
-_MODULE = None
 
 
 def _wamx():
-    """The binding, imported once."""
-    global _MODULE
-    if _MODULE is not None:
-        return _MODULE
     root = str(Path(__file__).resolve().parent.parent / "wam.cpp_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
     import wamx
 
-    _MODULE = wamx
     return wamx
 
 
