@@ -65,6 +65,8 @@ typedef enum wamx_type {
      * value j (low half) and value j + 16 (high half): sign, two exponent bits,
      * one mantissa bit, {0, .5, 1, 1.5, 2, 3, 4, 6}.  The layout of ggml's
      * block_mxfp4.  ne[0] is a multiple of 32, nb[0] = 17 the bytes of a block.
+     * Rows do not overlap and views keep the blocks in their rows: a transpose,
+     * or a permute that moves dim 0, is refused.
      * Read by MUL_MAT and LINEAR (as the weight), GET_ROWS and CPY; written by
      * CPY. */
     WAMX_TYPE_MXFP4 = 39,

@@ -1101,7 +1101,7 @@ static bool supports(const wamx_tensor * t) {
         case WAMX_OP_RESHAPE:
         case WAMX_OP_PERMUTE:
         case WAMX_OP_TRANSPOSE:
-            return true;
+            return !mx_turned(t);
         case WAMX_OP_DUP:
         case WAMX_OP_CONT:
         case WAMX_OP_CPY:
@@ -1109,9 +1109,9 @@ static bool supports(const wamx_tensor * t) {
                 // Quantise or dequantise rows of whole blocks, one shape.
                 const wamx_tensor * q = is_mxfp4(t) ? t : s0;
                 const wamx_tensor * v = is_mxfp4(t) ? s0 : t;
-                return t->op == WAMX_OP_CPY && float_type(v) && is_mxfp4(q) && wamx_are_same_shape(s0, t) &&
-                       rows_contig(s0) && rows_contig(t) && q->ne[0] % wamx_blck_size(q->type) == 0 &&
-                       v->nb[1] % es(v) == 0 && (q == s0 || wamx_is_contiguous(t));
+                return t->op == WAMX_OP_CPY && float_type(v) && mx_rows_whole(q) && wamx_are_same_shape(s0, t) &&
+                       rows_contig(v) && v->nb[1] % es(v) == 0 &&
+                       (q == s0 || (wamx_is_contiguous(t) && (!s1 || mx_rows_whole(s1))));
             }
             return ok_type(s0) && ok_type(t) && wamx_nelements(s0) == wamx_nelements(t);
         case WAMX_OP_ADD:
@@ -1140,10 +1140,9 @@ static bool supports(const wamx_tensor * t) {
         }
         case WAMX_OP_GET_ROWS:
             if (is_mxfp4(s0))
-                return rows_contig(s0) && s0->ne[0] % wamx_blck_size(s0->type) == 0 && s0->ne[2] == 1 &&
-                       s0->ne[3] == 1 && s0->ne[1] > 0 && s1 && s1->type == WAMX_TYPE_I32 && rows_contig(s1) &&
-                       wamx_nelements(s1) == s1->ne[0] && float_type(t) && t->ne[0] == s0->ne[0] &&
-                       t->ne[1] == s1->ne[0] && t->ne[2] == 1 && t->ne[3] == 1 && rows_contig(t) &&
+                return mx_rows_whole(s0) && s0->ne[2] == 1 && s0->ne[3] == 1 && s0->ne[1] > 0 && s1 &&
+                       s1->type == WAMX_TYPE_I32 && rows_contig(s1) && wamx_nelements(s1) == s1->ne[0] &&
+                       float_type(t) && t->ne[0] == s0->ne[0] && t->ne[1] == s1->ne[0] && t->ne[2] == 1 && t->ne[3] == 1 && rows_contig(t) &&
                        t->nb[1] % es(t) == 0;
             return ok_type(s0) && s1 && s1->type == WAMX_TYPE_I32 && rows_contig(s1) && t->ne[0] == s0->ne[0] &&
                    t->ne[1] == s1->ne[0] && t->ne[2] == s1->ne[1] && float_type(t);
@@ -1174,7 +1173,7 @@ static bool supports(const wamx_tensor * t) {
                 return false;
             if (tensor_is_tiled(s0)) return tiled_product_ok(s1) && wamx_is_contiguous(t);
             if (is_mxfp4(s0))
-                return s0->ne[0] > 0 && s0->ne[0] < 1 << 30 && s0->ne[0] % wamx_blck_size(s0->type) == 0 && rows_contig(s0) &&
+                return s0->ne[0] > 0 && s0->ne[0] < 1 << 30 && mx_rows_whole(s0) &&
                        (s1->type == WAMX_TYPE_BF16 || s1->type == WAMX_TYPE_F32) && rows_contig(s1) &&
                        s1->nb[1] % es(s1) == 0 && s1->nb[2] % es(s1) == 0 && s1->nb[3] % es(s1) == 0 &&
                        wamx_is_contiguous(t);

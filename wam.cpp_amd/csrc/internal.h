@@ -17,6 +17,12 @@ const char * check_qk_norm_rope(const wamx_tensor * t);
 const char * check_joint_attn(const wamx_tensor * t);
 const char * check_head_norm_rope(const wamx_tensor * t);
 const char * check_tree_attn(const wamx_tensor * t);
+// Whether t is rows of whole MXFP4 blocks: the blocks of a row one after another,
+// no row within another, no turned view (of 32 x 32 values it has the strides of
+// rows) on the way to the tensor.  Every reader and writer of the type asks this.
+bool mx_rows_whole(const wamx_tensor * t);
+// Whether view op t takes the blocks of an MXFP4 tensor out of their rows.
+bool mx_turned(const wamx_tensor * t);
 const char * check_modulation(const wamx_tensor * t);
 const char * check_euler_step(const wamx_tensor * t);
 const char * check_mlp_small(const wamx_tensor * t);

@@ -115,6 +115,28 @@ namespace wamx {
 // when the node is well formed, else the reason.
 static bool contig(const wamx_tensor * t) { return t && wamx_is_contiguous(t); }
 
+bool mx_turned(const wamx_tensor * t) {
+    return t->type == WAMX_TYPE_MXFP4 &&
+           (t->op == WAMX_OP_TRANSPOSE || (t->op == WAMX_OP_PERMUTE && t->op_params[0] != 0));
+}
+
+bool mx_rows_whole(const wamx_tensor * t) {
+    if (!t || t->type != WAMX_TYPE_MXFP4) return false;
+    const int64_t blck = wamx_blck_size(t->type);
+    const size_t size = wamx_type_size(t->type);
+    if (t->nb[0] != size || t->ne[0] % blck != 0) return false;
+    for (int i = 1; i < WAMX_MAX_DIMS; ++i)
+        if (t->ne[i] > 1 && t->nb[i] < size * (size_t) (t->ne[0] / blck)) return false;
+    int hops = 0;
+    for (; t; t = t->src[0]) {
+        const bool view = t->op == WAMX_OP_VIEW || t->op == WAMX_OP_RESHAPE || t->op == WAMX_OP_PERMUTE ||
+                          t->op == WAMX_OP_TRANSPOSE;
+        if (!view) return true;
+        if (mx_turned(t) || ++hops > 64) return false;
+    }
+    return true;
+}
+
 const char * check_linear(const wamx_tensor * t) {
     const wamx_tensor *w = t->src[0], *x = t->src[1], *bias = t->src[2], *res = t->src[3], *gate = t->src[4];
     const int32_t epi = t->op_params[0];
@@ -122,7 +144,7 @@ const char * check_linear(const wamx_tensor * t) {
     if ((!is_bf16(w) && !mx) || !x || (x->type != WAMX_TYPE_BF16 && x->type != WAMX_TYPE_F32)) return "types";
     if (w->ne[0] != x->ne[0] || w->ne[2] != 1 || w->ne[3] != 1 || x->ne[2] != 1 || x->ne[3] != 1) return "shapes";
     if (w->nb[0] != wamx_type_size(w->type) || x->nb[0] != wamx_type_size(x->type)) return "rows must be contiguous";
-    if (mx && (w->ne[0] % wamx_blck_size(w->type) != 0 || w->ne[0] >= 1 << 30)) return "rows of whole blocks, below 2^30";
+    if (mx && (!mx_rows_whole(w) || w->ne[0] >= 1 << 30)) return "rows of whole blocks, below 2^30";
     const int64_t M = w->ne[1], N = x->ne[1];
     if (epi < WAMX_EPI_NONE || epi > WAMX_EPI_BIAS_RESIDUAL) return "epilogue";
     if (epi != WAMX_EPI_NONE && (!is_bf16(bias) || bias->ne[0] != M || bias->nb[0] != 2)) return "bias";
@@ -558,6 +580,10 @@ wamx_tensor * wamx_permute(wamx_context * ctx, wamx_tensor * a, int axis0, int a
     for (int i = 0; i < 4; ++i) {
         if (ax[i] < 0 || ax[i] > 3 || seen[ax[i]]) return fail("wamx_permute");
         seen[ax[i]] = true;
+    }
+    if (a && axis0 != 0 && wamx_blck_size(a->type) > 1) {
+        set_errorf("wamx_permute: the blocks of %s stay in their rows", wamx_type_name(a->type));
+        return nullptr;
     }
     wamx_tensor * t = view_impl(ctx, a, 4, a->ne, 0);
     if (!t) return nullptr;
