@@ -350,7 +350,8 @@ WAMX_API wamx_tensor * wamx_rms_norm_bf16_f32(wamx_context * ctx, wamx_tensor * 
  *   ancestors: parents I32 [T, B] holds each token's parent, -1 at the root.
  *   Any other value outside [0, T) marks a slot without a token: nothing sees
  *   it and its result is zero.  A sequence whose past[b] is outside
- *   [0, rows - T] gets zeros.  T 1 to 256.  Output bf16 [ne={dh*H, T, B}].
+ *   [0, rows - T] gets zeros.  A token all of whose scores are -Inf gets NaN, as
+ *   the softmax has it.  T 1 to 256.  Output bf16 [ne={dh*H, T, B}].
  */
 WAMX_API wamx_tensor * wamx_linear(wamx_context * ctx, wamx_tensor * w, wamx_tensor * x, wamx_tensor * bias,
                                    int32_t epilogue, wamx_tensor * residual, wamx_tensor * gate);

@@ -428,16 +428,16 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
         const int r = i * 16 + c16, row = row0 + r;
         const float sum = (sm[0][r] + sm[1][r]) + (sm[2][r] + sm[3][r]);
         if (row >= rows) continue;
-        const bool none = !token[i] || (sum == 0.0f && m[i] == -INFINITY);
+        // Scores that are all -Inf leave 0 / 0, which is NaN.
+        const bool none = !token[i] || n == 0;
         const int d0 = wave * (DH / 4) + 4 * g;
         if (p.po) {
             const int64_t at = ((int64_t) u * p.kv_heads + hk) * rows + row;
 #pragma unroll
             for (int d = 0; d < DT; ++d) *(f32x4_t *) (p.po + at * DH + d0 + d * 16) = o[i][d];
             if (wave == 0 && g == 0) {
-                // A sum that is NaN must outlive a maximum that no score raised.
-                p.pml[2 * at] = none ? -INFINITY : m[i] == -INFINITY ? 0.0f : m[i];
-                p.pml[2 * at + 1] = none ? 0.0f : sum;
+                p.pml[2 * at] = m[i];
+                p.pml[2 * at + 1] = sum;
             }
         } else {
             const float inv = none ? 0.0f : 1.0f / sum;
@@ -698,14 +698,14 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
         const float sum = sum_xor32(sum_xor16(l[i]));
         if (row >= rows) continue;
         const int pr = parents[tok[i]];
-        const bool none = !(pr >= -1 && pr < p.tq) || (sum == 0.0f && m[i] == -INFINITY);
+        const bool none = !(pr >= -1 && pr < p.tq) || n == 0;
         if (p.po) {
             const int64_t at = ((int64_t) u * p.kv_heads + hk) * rows + row;
 #pragma unroll
             for (int d = 0; d < DT; ++d) *(f32x4_t *) (p.po + at * DH + d * 16 + 4 * g) = o[i][d];
             if (g == 0) {
-                p.pml[2 * at] = none ? -INFINITY : m[i] == -INFINITY ? 0.0f : m[i];
-                p.pml[2 * at + 1] = none ? 0.0f : sum;
+                p.pml[2 * at] = m[i];
+                p.pml[2 * at + 1] = sum;
             }
         } else {
             const float inv = none ? 0.0f : 1.0f / sum;
@@ -737,6 +737,7 @@ __global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int row_part
     const int64_t b = bz / (uint32_t) p.kv_heads;
     const int hk = (int) (bz - (uint32_t) b * (uint32_t) p.kv_heads);
     const TreeUnit unit = tree_unit(p, 0, (int) b);
+    const int parent = p.parents[b * p.tq + row % p.tq];
     const int64_t step = (int64_t) p.kv_heads * rows, at = unit.first * step + hk * rows + row;
     float m = -INFINITY, sum = 0.0f;
     f32x4_t v = {0, 0, 0, 0};
@@ -761,8 +762,9 @@ __global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int row_part
         m = top;
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
-            // A unit without a slot of this row has no part (it may hold NaN).
-            if (ms[k] == -INFINITY) continue;
+            // A unit without a finite score has weight zero: 0 times its results,
+            // which hold NaN where 0 met an Inf or NaN value.
+            if (s0 + k * BY >= unit.count) continue;
             const float f = __builtin_amdgcn_exp2f(ms[k] - bm);
             sum += ls[k] * f;
             v += o[k] * f;
@@ -793,7 +795,7 @@ __global__ __launch_bounds__(256) void tree_attn_join(TreeParams p, int row_part
     } else if (first + gr >= rows) {
         return;
     }
-    const bool none = m == -INFINITY;
+    const bool none = !(parent >= -1 && parent < p.tq) || unit.slots == 0;
     const float inv = none ? 0.0f : 1.0f / sum;
     uint16_t * y = p.out + ((b * p.tq + row % p.tq) * p.heads + hk * group + row / p.tq) * DH + piece * 4;
     *(uint32_t *) y = none ? 0u : pack_bf16x2(v[0] * inv, v[1] * inv);
