@@ -376,7 +376,7 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
         for (int i = 0; i < RG; ++i) t[i] = mx_load(w[i] + o);
     };
     auto load_x = [&](int s) {
-        const uint32_t xo = (uint32_t) ((4 * s + (r >> 2) < p.kb ? s * 128 : -r * 8) * xs);  // past the row: its start
+        const uint32_t xo = (uint32_t) (4 * s + (r >> 2) < p.kb ? s * 128 : -r * 8) * (uint32_t) xs;  // past the row: its start
 #pragma unroll
         for (int j = 0; j < NT * 4; ++j)
 #pragma unroll
@@ -852,14 +852,15 @@ hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     p.epi = a.epi;
     p.steps = (p.kb + 3) / 4;
     const bool xf32 = a.x_type == WAMX_TYPE_F32;
-    // Tokens in parts that a grid takes.  f32 activations of more than 32: rounded
-    // once into half of the workspace, as many rows at a time as it holds.
-    const bool round = xf32 && a.N > 32;
+    // Tokens in parts that a grid takes.  Rows so long or so far apart that 64 of
+    // them pass 32-bit offsets go one by one.
+    int64_t part = std::max(a.ldx, a.K) > 1 << 23 ? 1 : 1 << 20;
+    // f32 activations of more than 32: rounded once into half of the workspace, as
+    // many rows at a time as it holds; where it holds none, 32 on their way.
     const size_t row = (size_t) a.K * 2, half = a.ws ? a.ws_bytes / 2 : 0;
-    // Rows so far apart that 64 of them pass 32-bit offsets go one by one.
-    int64_t part = a.ldx > 1 << 23 ? 1 : 1 << 20;
+    const bool round = xf32 && a.N > 32 && part > 1 && row <= half;
     if (round) part = std::min<int64_t>(std::min<int64_t>(part, (int64_t) (half / row)), 0x3fffffff / (a.K / 8) * 256);
-    if (part < 1) return hipErrorInvalidValue;
+    else if (xf32) part = std::min<int64_t>(part, 32);
     for (int64_t n = 0; n < a.N; n += part) {
         MxParams q = p;
         q.N = std::min(part, a.N - n);
