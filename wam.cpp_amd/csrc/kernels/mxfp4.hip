@@ -749,9 +749,11 @@ static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipSt
     // tiles 19.9).
     const bool near = std::max(p.ws, p.ldx * 2) < (1ll << 23);  // a tile's 256 rows within 32-bit offsets
     const bool few = p.N <= 48 || (p.N <= 64 && groups <= 512) || !near;
+    // Four token tiles leave registers for two groups.
+    const int most = p.N > 48 ? 2 : 4;
     int rg = 1, splits = 1;
     int64_t least = 0;
-    for (int c = 1; c <= 4; c *= 2) {
+    for (int c = 1; c <= most; c *= 2) {
         const int64_t t = (groups + 256 * c - 1) / (256 * c) * (2 * c + (std::min<int64_t>(p.N, 64) + 15) / 16);
         if (least && t > least) continue;
         least = t;
@@ -765,7 +767,7 @@ static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipSt
         // Long rows, few of them: four K splits of 256 workgroups in all
         // (2048 x 64 x 14336: 18 us against 26, 4096 x 48 x 14336: 22 against 28).
         splits = 4;
-        rg = groups > 128 ? 4 : groups > 64 ? 2 : 1;
+        rg = std::min(most, groups > 128 ? 4 : groups > 64 ? 2 : 1);
     }
     p.steps = (steps + splits - 1) / splits;
     splits = (steps + p.steps - 1) / p.steps;
@@ -856,11 +858,11 @@ hipError_t launch_mx_product(const MxArgs & a, hipStream_t s) {
     // them pass 32-bit offsets go one by one.
     int64_t part = std::max(a.ldx, a.K) > 1 << 23 ? 1 : 1 << 20;
     // f32 activations of more than 32: rounded once into half of the workspace, as
-    // many rows at a time as it holds; where it holds none, 32 on their way.
-    const size_t row = (size_t) a.K * 2, half = a.ws ? a.ws_bytes / 2 : 0;
-    const bool round = xf32 && a.N > 32 && part > 1 && row <= half;
+    // many rows at a time as it holds (two at least); single rows on their way.
+    const size_t row = (size_t) a.K * 2, half = a.ws_bytes / 2;
+    static_assert(kBackendWorkspaceBytes / 2 >= (2u << 23), "a row of 2^23 values fits");
+    const bool round = xf32 && a.N > 32 && part > 1;
     if (round) part = std::min<int64_t>(std::min<int64_t>(part, (int64_t) (half / row)), 0x3fffffff / (a.K / 8) * 256);
-    else if (xf32) part = std::min<int64_t>(part, 32);
     for (int64_t n = 0; n < a.N; n += part) {
         MxParams q = p;
         q.N = std::min(part, a.N - n);

@@ -226,7 +226,7 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// NR tiles of 16 rows for a workgroup, slots in tiles of 64: wave w takes slots
+// All rows, up to NR tiles of 16, for a workgroup; slots in tiles of 64: wave w takes slots
 // 16w .. of a tile for the scores of all rows, and DH / 4 of the result's
 // dimensions for all rows and slots, so every K and V element is loaded once,
 // by one wave, into the registers that feed its matrix operand.  The rows (Q)
@@ -243,12 +243,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
-    // Row tiles of one unit are eight workgroups apart: the same XCD, whose L2
-    // then holds the slots they share.
-    const int rt = (rows + R - 1) / R;
-    const uint32_t id = blockIdx.x, at8 = id / (uint32_t) (8 * rt) * 8 + id % 8;
-    const int row0 = (int) (id / 8 % (uint32_t) rt) * R;
-    const int hk = (int) (at8 / (uint32_t) p.units), u = (int) at8 - hk * p.units;
+    const int hk = (int) (blockIdx.x / (uint32_t) p.units), u = (int) blockIdx.x - hk * p.units;
     if (hk >= p.kv_heads) return;
     const TreeUnit unit = tree_unit(p, u);
     if (unit.b < 0) return;
@@ -285,7 +280,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     // rows of an operand read lie in different banks.
     auto qswz = [](int r) { return DH == 64 ? (r >> 1) & 7 : r & 15; };
     for (int e = threadIdx.x; e < R * QCH; e += kTreeWaves * 64) {
-        const int r = e / QCH, c = e % QCH, row = min(row0 + r, rows - 1);
+        const int r = e / QCH, c = e % QCH, row = min(r, rows - 1);
         const uint16_t * qr = p.q + (((int64_t) b * p.heads + hk * group + row / p.tq) * p.tq + row % p.tq) * DH;
         *(bf16x8_t *) (qs + r * DH + (c ^ qswz(r)) * 8) = tree_q(p, qr + c * 8);
     }
@@ -293,7 +288,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     bool token[NR];  // a place that holds a token
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        tok[i] = min(row0 + i * 16 + c16, rows - 1) % p.tq;
+        tok[i] = min(i * 16 + c16, rows - 1) % p.tq;
         const int pr = parents[tok[i]];
         token[i] = pr >= -1 && pr < p.tq;
     }
@@ -401,7 +396,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 if (!(path[i] >> a & 1)) continue;
-                const int row = min(row0 + i * 16 + c16, rows - 1);
+                const int row = min(i * 16 + c16, rows - 1);
                 const float pr =
                     tree_weight(p, b, hk * group + row / p.tq, tok[i], kb - g * 8 + slot * DH, DH, m[i]);
 #pragma unroll
@@ -425,8 +420,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        const int r = i * 16 + c16, row = row0 + r;
-        const float sum = (sm[0][r] + sm[1][r]) + (sm[2][r] + sm[3][r]);
+        const int row = i * 16 + c16;
+        const float sum = (sm[0][row] + sm[1][row]) + (sm[2][row] + sm[3][row]);
         if (row >= rows) continue;
         // Scores that are all -Inf leave 0 / 0, which is NaN.
         const bool none = !token[i] || n == 0;
@@ -465,7 +460,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
 // taken out once, on its way to LDS (100 tokens of 2 x 8 heads of 256 over 4000
 // slots 34 us, by every wave that reads it 43).
 template <int DH, int NR, int W>
-__global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreeParams p) {
+__global__ __launch_bounds__(W * 64, 1) void tree_attn_many(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 16, TILE = 64, R = W * NR * 16, QCH = DH / 8;
     constexpr int KN = TILE * QCH / (W * 64), VN = DH * 8 / (W * 64);  // 16-byte pieces of a thread
     __shared__ __align__(16) uint16_t kt_lds[2][TILE * DH];
@@ -476,6 +471,8 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void tree_attn_many(TreePar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     const int group = p.heads / p.kv_heads, rows = group * p.tq;
+    // Row tiles of one unit are eight workgroups apart: the same XCD, whose L2
+    // then holds the slots they share.
     const int rt = (rows + R - 1) / R;
     const uint32_t id = blockIdx.x, at8 = id / (uint32_t) (8 * rt) * 8 + id % 8;
     const int row0 = (int) (id / 8 % (uint32_t) rt) * R + wave * NR * 16;
@@ -810,7 +807,7 @@ static void plan(TreeParams & p, const TreeArgs & a, int64_t row_tiles, int64_t 
     const int64_t rows = a.heads / a.kv_heads * a.tq, tiles = (a.capacity + kTreeTile - 1) / kTreeTile;
     int64_t units = std::min<int64_t>(wgs / (a.kv_heads * row_tiles), a.batch * std::max<int64_t>(tiles / kTreeLeast, 1));
     const size_t per = (size_t) (a.kv_heads * rows) * (size_t) (a.head_dim + 2) * 4;
-    if (!a.ws || a.ws_bytes / per < (size_t) units) units = a.ws ? (int64_t) (a.ws_bytes / per) : 0;
+    units = std::min<int64_t>(units, (int64_t) (a.ws_bytes / per));
     p.even = a.batch > 64 || (uint64_t) units * (uint64_t) tiles * (uint64_t) a.batch > 0xffffffffull;
     if (p.even) units = units / a.batch * a.batch;
     p.units = (int32_t) std::max<int64_t>(units, a.batch);
@@ -861,8 +858,8 @@ hipError_t launch_tree_attn(const TreeArgs & a, hipStream_t s) {
     // Wide reads of q, k and V^T, and result stores of two values.
     if (((uintptr_t) a.q | (uintptr_t) a.k | (uintptr_t) a.vt) % 16 != 0 || (uintptr_t) a.out % 4 != 0)
         return hipErrorInvalidValue;
-    if (a.tq > kTreeMax || a.batch > 0x7fffffff / std::max<int64_t>(a.kv_heads, 1) || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.vt_ld % 8 != 0 ||
-        a.vt_ld < a.capacity || a.capacity <= 0 || a.capacity > 0x7fffffff)
+    if (a.tq > kTreeMax || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 ||
+        a.batch > 0x7fffffff / a.kv_heads || a.vt_ld % 8 != 0 || a.vt_ld < a.capacity || a.capacity <= 0 || a.capacity > 0x7fffffff)
         return hipErrorInvalidValue;
     TreeParams p{};
     p.q = (const uint16_t *) a.q;
