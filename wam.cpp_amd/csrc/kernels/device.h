@@ -93,6 +93,15 @@ __device__ __forceinline__ float block_sum(float v, float * red) {
     return t;
 }
 
+// A barrier that waits for this wave's LDS accesses alone: loads into registers
+// stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float load_as_f32(const void * p, int32_t type, int64_t i) {
     if (type == 0) return ((const float *) p)[i];
     if (type == 30) return bf16_to_f32(((const uint16_t *) p)[i]);

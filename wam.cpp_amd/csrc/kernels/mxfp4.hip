@@ -27,15 +27,6 @@ struct __attribute__((packed, aligned(1))) any8 {
     uint32_t v[2];
 };
 
-// A barrier that waits for this wave's LDS accesses alone: loads into registers
-// stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // A block read as the five aligned dwords that hold its 17 bytes, `mis` bytes
 // into the first (every dword holds a byte of the block, so none lies outside
 // the tensor's pages).  As 16 + 1 bytes at their odd addresses the few-token

@@ -217,15 +217,6 @@ __device__ __forceinline__ void tree_range(int64_t n, int i, int count, int64_t 
     t1 = t0 + q + ((uint32_t) i < r);
 }
 
-// A barrier that waits for this wave's LDS accesses alone: loads into registers
-// stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // All rows, up to NR tiles of 16, for a workgroup; slots in tiles of 64: wave w takes slots
 // 16w .. of a tile for the scores of all rows, and DH / 4 of the result's
 // dimensions for all rows and slots, so every K and V element is loaded once,
