@@ -68,10 +68,10 @@ constexpr int kHnThreads = 256, kHnTile = 64;
 // part, whose workgroups come first, transposes tiles of 64 slots through LDS;
 // tiles begin at multiples of 64, so eight slots are one aligned store.
 //
-// The bytes bound it: 4002 tokens of (32 + 8 + 8) heads of 128 take 23 us, 4.3
-// TB/s with the launch; one token 5 us, which is a launch and three dependent
-// reads.  With 16-byte pieces, whose halves' partners lie in other lanes, the
-// exchanges and twice the angles took 31.6 us.
+// The bytes bound it: 4002 tokens of (32 + 8 + 8) heads of 128 take 23 to 25 us,
+// 3.9 to 4.3 TB/s with the launch; one token 4.5 us, which is a launch and three
+// dependent reads.  With 16-byte pieces, whose halves' partners lie in other
+// lanes, the exchanges and twice the angles took 31.6 us.
 template <int DH>
 __global__ __launch_bounds__(kHnThreads) void head_norm_rope(HeadNormParams p) {
     constexpr int LPH = DH / 8, HPW = 64 / LPH;

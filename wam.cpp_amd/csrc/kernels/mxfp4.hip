@@ -30,8 +30,8 @@ struct __attribute__((packed, aligned(1))) any8 {
 // A block read as the five aligned dwords that hold its 17 bytes, `mis` bytes
 // into the first (every dword holds a byte of the block, so none lies outside
 // the tensor's pages).  As 16 + 1 bytes at their odd addresses the few-token
-// products took 7.1 and 32 us where these take 5.3 and 27 (4096 x 1 x 4096,
-// 14336 x 48 x 4096).  Blocks four apart have one `mis`.
+// products took 34% and 19% longer (4096 x 1 x 4096, 14336 x 48 x 4096).  Blocks
+// four apart have one `mis`.
 struct __attribute__((packed, aligned(4))) dwords4 {
     uint32_t v[4];
 };
@@ -168,8 +168,8 @@ __global__ __launch_bounds__(kQThreads) void mx_quantize(const T * __restrict__ 
 // elements; qs the byte stride of packed rows (row_blocks * 17 when they follow
 // each other); rows (nullable) picks row rows[r] of `qrows` packed rows
 // (negative or past the end: NaN).  Bound by its writes: 14336 x 4096 values to
-// f32 44 us, 6.1 TB/s over reads and writes that the caches still hold; with
-// the quantisation that precedes it 116 us, 4.6 TB/s.
+// f32 71 us (bf16 34), quantised from it 50 (bf16 26); one after the other 116,
+// 4.3 TB/s (bf16 58).
 template <typename T>
 __global__ __launch_bounds__(kQThreads) void mx_dequantize(const uint8_t * __restrict__ q, int64_t qs,
                                                            const int32_t * __restrict__ rows, int64_t qrows,
@@ -315,8 +315,13 @@ __device__ __forceinline__ bf16x8_t mx_pair(uint32_t lo0, uint32_t lo1, uint32_t
     return u.v;
 }
 
-// Few tokens: the weight bytes bound it, so every one is read once, in
-// 16-byte pieces, and goes straight into matrix operands.  A workgroup takes
+// Few tokens: every byte of the weight is read once, in 16-byte pieces, and goes
+// straight into matrix operands.  What it takes beyond those bytes' time is not
+// the expansion of the codes (with the bits as they are instead, which computes
+// something else, every size takes as long) but x, which each workgroup reads and
+// passes through LDS (without: 14336 x 48 x 4096 13.4 us for 18.1, 20000 x 1 x
+// 4096 14.8 for 17.4, where all 16 token rows are copies of the one), and the
+// latency of the few K steps that a wave has.  A workgroup takes
 // RG groups of 16 weight rows and NT tiles of 16 tokens; its waves take the K
 // steps of 128 in turn (a row's 68 bytes of a step lie next to the next
 // wave's) and their sums meet in LDS in wave order.  Lane (r, g) holds block g
@@ -356,8 +361,9 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
     uint4 * mine = (uint4 *) (lds + wave * XB);
 
     // x of the next step is requested when this one's lies in LDS, the weights
-    // kMxAhead steps before their use (one: 14336 x 48 x 4096 19.1 us for 18.5,
-    // three: spills).
+    // kMxAhead steps before their use (one: 14336 x 48 x 4096 19.0 us for 18.1,
+    // 14336 x 32 x 4096 16.2 for 15.8, but 20000 x 1 x 4096 17.0 for 17.7; three:
+    // spills).
     MxBlock wr[kMxAhead + 1][RG];
     any16 xr[NT * 4][XF32 ? 2 : 1];
     auto load_w = [&](int s, MxBlock * t) {
@@ -476,8 +482,8 @@ __global__ __launch_bounds__(kMxWaves * 64) void mx_few(MxParams p) {
 
 // Many tokens: WM waves along the weight rows by WN along the tokens, each RG x
 // NT tiles of 16 x 16.  Every wave expands its rows' codes itself, so 128 x 128
-// tiles take 4 x 2 waves of 2 x 4 tiles (10250 x 333 x 2048: 28.9 us, 2 x 4
-// waves of 4 x 2 tiles 30.5).  The weight stays in its 4 bits down to the
+// tiles take 4 x 2 waves of 2 x 4 tiles (10250 x 333 x 2048: 24.6 us, 2 x 4
+// waves of 4 x 2 tiles 28.6).  The weight stays in its 4 bits down to the
 // register that becomes the operand: a step of 128 values is 4 blocks a row,
 // whose codes are put into the order of their values on the way to LDS and lie
 // there as [block][row][g], so that a wave's read of dword g of its rows is 256
@@ -698,9 +704,9 @@ static void launch_tile(const MxParams & p, int splits, hipStream_t s) {
 // 1.4 alone and 2.4 in pairs, 64 x 64 0.69, 1.03 and with five 2.5); the planes
 // of the splits are written and read at 4 TB/s, and they cost one more launch.
 // Modelled and measured: 14336 x 128 x 4096 in 128 x 128 tiles and 2 splits 35
-// and 34, in 64 x 64 unsplit 38 and 37; 4096 x 128 x 4096 in 64 x 64 and 4
-// splits 19 and 21; 4096 x 70 x 14336 in 128 x 128 and 8 splits 29 and 30, in
-// 64 x 64 and 4 splits 41 and 36.
+// and 33, in 64 x 64 unsplit 38 and 38; 4096 x 128 x 4096 in 64 x 64 and 4
+// splits 19 and 20; 4096 x 70 x 14336 in 128 x 128 and 8 splits 29 and 29, in
+// 64 x 64 and 4 splits 41 and 37.
 struct TilePlan {
     int kind, splits;
 };
@@ -733,11 +739,11 @@ static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipSt
     const int64_t groups = (p.M + 15) / 16;
     // Few tokens: groups of 16 rows to a workgroup by how many workgroups a CU
     // then has to run and what each costs, two for a group's weights and one for
-    // a tile's x (us with 1, 2 and 4 groups: 4096 x 1 x 4096 6.3, 8.0, 12.1;
-    // 20000 x 1 x 4096 21.5, 17.6, 22.7; 14336 x 32 x 4096 24.0, 19.9, 15.7;
-    // 14336 x 48 x 4096 35.8, 24.0, 18.3).  49 to 64 tokens come here while 512
-    // groups, a workgroup per CU, hold the rows (6400 x 64 x 4096 15.2 us, in
-    // tiles 19.9).
+    // a tile's x (us with 1, 2 and 4 groups: 4096 x 1 x 4096 6.2, 7.8, 12.0;
+    // 20000 x 1 x 4096 21.2, 17.7, 22.5; 14336 x 32 x 4096 24.2, 20.0, 15.8;
+    // 14336 x 48 x 4096 35.7, 24.0, 18.1).  49 to 64 tokens come here while 512
+    // groups, a workgroup per CU, hold the rows (6400 x 64 x 4096 14.6 us, in
+    // tiles 20.4).
     const bool near = std::max(p.ws, p.ldx * 2) < (1ll << 23);  // a tile's 256 rows within 32-bit offsets
     const bool few = p.N <= 48 || (p.N <= 64 && groups <= 512) || !near;
     // Four token tiles leave registers for two groups.
@@ -756,7 +762,8 @@ static void run_product(MxParams p, bool xf32, void * ws, size_t ws_bytes, hipSt
         splits = plan.splits;
     } else if (p.N > 32 && steps >= 96 && groups <= 256 && 16 * (size_t) p.N * (size_t) p.M <= ws_bytes) {
         // Long rows, few of them: four K splits of 256 workgroups in all
-        // (2048 x 64 x 14336: 18 us against 26, 4096 x 48 x 14336: 22 against 28).
+        // (2048 x 64 x 14336: 17.5 us, unsplit in as many row groups 39; 4096 x 48
+        // x 14336: 20.7, 47).
         splits = 4;
         rg = std::min(most, groups > 128 ? 4 : groups > 64 ? 2 : 1);
     }

@@ -223,8 +223,16 @@ __device__ __forceinline__ void tree_range(int64_t n, int i, int count, int64_t 
 // by one wave, into the registers that feed its matrix operand.  The rows (Q)
 // and the probabilities lie in LDS.  K of the next tile is requested when this
 // tile's scores are done and V when its product is.  The slots' bytes bound it:
-// one token of 2 x 16 heads of 64 (4 key heads) over 100000 slots 37 to 39 us
+// one token of 2 x 16 heads of 64 (4 key heads) over 100000 slots 36 to 39 us
 // with the join, 4.6 to 4.9 TB/s.
+//
+// The probabilities are rounded to bf16, the only operand type that V's matrix
+// instruction takes beside it, here and in tree_attn_many; their sum is of the
+// unrounded ones, in f32, as are maxima and results.  Each is off by at most 2^-8
+// of itself, independently, so a result by at most 2^-8 sum p |v| / sum p and
+// typically by 1.5e-3 of itself, as much as the rounding of the result to bf16
+// alone (against 64 bits: 2.3e-3 together, 1.7e-3 with exact probabilities).  A
+// second operand with the rounded-off parts would double the products of V.
 template <int DH, int NR>
 __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams p) {
     constexpr int KC = DH / 32, DT = DH / 64, TILE = 64, R = NR * 16, QCH = DH / 8;
@@ -444,9 +452,9 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_attn_rows(TreeParams 
 // half) eight consecutive slots in its registers: the operand of O^T = V^T P^T
 // as it stands.  K and V^T tiles of 64 slots go through registers into one of
 // two LDS buffers while the other is used; one barrier a tile.  A tile of 128
-// dimensions takes 5 k cycles for 2 k each of MFMA, exponentials with their sums
-// and LDS reads: 64 tokens of 4 x 32 heads (8 key heads) over 16000 slots 85 us
-// with the join, 0.64 PFLOP/s.  Two row tiles a wave in eight waves; four in four
+// dimensions takes 5 k cycles, of which MFMA fill 34%, other vector instructions
+// 32% and LDS 21%: 64 tokens of 4 x 32 heads (8 key heads) over 16000 slots 87 us
+// with the join, 0.63 PFLOP/s (102 call after call, where the clock sinks).  Two row tiles a wave in eight waves; four in four
 // waves of 512 registers 106 us, two in four 99.  What is not to be seen of V is
 // taken out once, on its way to LDS (100 tokens of 2 x 8 heads of 256 over 4000
 // slots 34 us, by every wave that reads it 43).
@@ -831,13 +839,18 @@ static hipError_t launch(void (*kernel)(TreeParams), int R, int threads, int64_t
     return hipGetLastError();
 }
 
-// As many workgroups as it takes to keep 16 MB of slots requested, where the
-// registers let them run together (one token of 4 x 4 heads of 64, 100000 slots:
-// 256 workgroups 62 us, 512 39, 768 36; 8 tokens of 4 x 8 heads of 128: 39, 34,
-// 35; 33 tokens of 8 heads of 256: 35, 37, 39).
+// Workgroups that keep enough of the slots requested, 256, 512 and 768 of them
+// measured: narrow heads request little each (us, one token of 4 x 4 heads of 64
+// over 100000 slots: 111, 66, 64; of 2 x 16 / 4 heads: 58, 38, 36), wider ones do
+// with 512 (8 tokens of 4 x 8 heads of 128 over 8000: 32, 28, 29; 8 tokens of 16 /
+// 8 heads of 256 over 20000: 41, 41, 42).  33 to 48 rows of 256 have results so
+// large, 48 KB a unit, that twice the units cost more in the join than they
+// bring (40 tokens of 8 heads over 16000: 39, 41, 53; 2 x 12 tokens of 16 / 4
+// heads over 12000: 33, 37, 44; 3 x 33 of 8 over 5000: 36, 38, 49).
 template <int DH, int NR>
 static hipError_t run_rows(TreeParams & p, const TreeArgs & a, hipStream_t s) {
-    return launch<DH>(tree_attn_rows<DH, NR>, NR * 16, kTreeWaves * 64, DH == 64 ? 768 : NR * DH == 768 ? 256 : 512, p, a, s);
+    constexpr int kWorkgroups = DH == 64 ? 768 : DH == 256 && NR > 2 ? 256 : 512;
+    return launch<DH>(tree_attn_rows<DH, NR>, NR * 16, kTreeWaves * 64, kWorkgroups, p, a, s);
 }
 template <int DH, int NR, int W>
 static hipError_t run_many(TreeParams & p, const TreeArgs & a, hipStream_t s) {
